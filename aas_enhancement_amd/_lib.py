@@ -111,8 +111,27 @@ SIGNATURES = {
     "aas_began_step": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, ctypes.c_double, ctypes.c_double, ctypes.c_double],
     "aas_lmfb320_fwd": [c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_vp],
     "aas_lmfb_fwd": [c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_vp, c_vp, c_vp],
+    "aas_causal_conv1d_fwd": [c_vp, c_int, c_int, c_int, c_int, c_int, c_vp, c_i64, c_i64, c_vp, c_vp, c_int, c_vp, c_vp, c_vp],
+    "aas_causal_conv1d_bwd_ws_bytes": [c_int, c_int, c_int, c_int],
+    "aas_causal_conv1d_bwd": [c_vp, c_int, c_int, c_int, c_int, c_int, c_vp, c_i64, c_i64, c_vp, c_vp, c_int, c_vp, c_vp, c_i64, c_i64,
+                              c_vp, c_vp, c_vp, c_vp],
+    "aas_ssm_scan_fwd_ws_bytes": [c_int, c_int, c_int, c_int, c_int],
+    "aas_ssm_scan_fwd": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp],
+    "aas_ssm_scan_bwd_ws_bytes": [c_int, c_int, c_int, c_int, c_int],
+    "aas_ssm_scan_bwd": [c_vp, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp],
+    "aas_residual_norm_fwd": [c_vp, c_int, c_int, c_i64, c_int, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_f32, c_int, c_int, c_i64, c_i64,
+                              c_vp, c_vp, c_vp, c_vp, c_vp],
+    "aas_residual_norm_bwd_ws_bytes": [c_i64, c_int],
+    "aas_residual_norm_bwd": [c_vp, c_int, c_int, c_i64, c_int, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_int, c_int,
+                              c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp],
+    "aas_gated_norm_fwd": [c_vp, c_int, c_i64, c_int, c_int, c_vp, c_i64, c_vp, c_i64, c_vp, c_f32, c_int, c_vp],
+    "aas_gated_norm_bwd_ws_bytes": [c_i64, c_int, c_int],
+    "aas_gated_norm_bwd": [c_vp, c_int, c_i64, c_int, c_int, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_f32, c_int, c_vp, c_vp, c_vp, c_vp],
+    "aas_dropout": [c_vp, c_int, c_i64, c_vp, c_vp, c_int, c_i64, c_i64, c_vp, c_vp],
 }
-_RESTYPES = {"aas_last_error": ctypes.c_char_p, "aas_rnn_sync_bytes": c_sz, "aas_rnn_xchg_bytes": c_sz}
+_RESTYPES = {"aas_last_error": ctypes.c_char_p, "aas_rnn_sync_bytes": c_sz, "aas_rnn_xchg_bytes": c_sz, "aas_causal_conv1d_bwd_ws_bytes": c_sz,
+             "aas_ssm_scan_fwd_ws_bytes": c_sz, "aas_ssm_scan_bwd_ws_bytes": c_sz, "aas_residual_norm_bwd_ws_bytes": c_sz,
+             "aas_gated_norm_bwd_ws_bytes": c_sz}
 
 
 def lib():

@@ -1,0 +1,185 @@
+// Root-mean-square norm with a gate, per group of cg channels, forward and backward.  With G = z sigmoid(z), G' its derivative:
+//   norm_first = 0: v = x G, y = hat w;      norm_first = 1: v = x, y = hat w G;      hat = v rstd, rstd = 1 / sqrt(mean(v^2) + eps);
+//   g = dy w (G),  dv = rstd (g - hat mean(g hat));   dx = dv G, dz = dv x G', dw = sum dy hat   |   dx = dv, dz = dy hat w G', dw = sum dy hat G.
+// HBM-bound: every tensor once; the backward pass forms the statistics again from x and z, which it reads anyway.
+#include "norm_rows.h"
+
+namespace {
+
+__device__ __forceinline__ float gate_of(float z, float& slope) {
+    const float s = sigm(z);
+    slope = s * fmaf(z, 1.f - s, 1.f);
+    return z * s;
+}
+
+template <class T, int TPR, int NV, bool VEC, bool FIRST>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void gated_fwd_kernel(int64_t rows, int C, int cg, int groups, const T* __restrict__ x, int64_t x_ld,
+                                                                           const T* __restrict__ z, int64_t z_ld, const float* __restrict__ w, float eps,
+                                                                           T* __restrict__ y) {
+    constexpr int RPB = TPR == 64 ? 4 : 1;
+    __shared__ float s[TPR / 64][2];
+    const int l = threadIdx.x % TPR;
+    const int64_t id = (int64_t)blockIdx.x * RPB + (RPB > 1 ? threadIdx.x / TPR : 0);
+    const int64_t row = id / groups;
+    const int base = (int)(id - row * groups) * cg;
+    if (row >= rows) return;
+    f32x4 v[NV], gt[NV];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * TPR + l) * 4, n = cg - c;
+        v[i] = load4n<T, VEC>(x + row * x_ld + base + c, n);
+        gt[i] = load4n<T, VEC>(z + row * z_ld + base + c, n);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            gt[i][j] *= sigm(gt[i][j]);
+            if (!FIRST) v[i][j] *= gt[i][j];
+            if (j >= n) v[i][j] = 0.f;
+            s1 = fmaf(v[i][j], v[i][j], s1);
+        }
+    }
+    row_sum2<TPR>(s1, s2, s);
+    const float rstd = 1.f / sqrtf(s1 / (float)cg + eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * TPR + l) * 4, n = cg - c;
+        const f32x4 wv = w ? load4n<float, VEC>(w + base + c, n) : f32x4{1.f, 1.f, 1.f, 1.f};
+        f32x4 o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            o[j] = v[i][j] * rstd * wv[j];
+            if (FIRST) o[j] *= gt[i][j];
+        }
+        store4n<T, VEC>(y + row * C + base + c, o, n);
+    }
+}
+
+template <class T, int TPR, int NV, bool VEC, bool FIRST>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void gated_bwd_kernel(int64_t rows, int C, int cg, const T* __restrict__ dy, int64_t dy_ld,
+                                                                           const T* __restrict__ x, int64_t x_ld, const T* __restrict__ z, int64_t z_ld,
+                                                                           const float* __restrict__ w, float eps, T* __restrict__ dx, T* __restrict__ dz,
+                                                                           float* __restrict__ part) {
+    constexpr int RPB = TPR == 64 ? 4 : 1;
+    __shared__ float s[TPR / 64][2];
+    __shared__ __align__(16) float cols[TPR == 64 ? 4 * NV * 256 : 4];
+    const int l = threadIdx.x % TPR, base = blockIdx.y * cg;           // a workgroup stays in one group: its threads own columns
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f}, one = {1.f, 1.f, 1.f, 1.f};
+    f32x4 aw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) aw[i] = zero;
+    const float inv = 1.f / (float)cg;
+    for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < rows; row0 += (int64_t)gridDim.x * RPB) {
+        const int64_t row = row0 + (RPB > 1 ? threadIdx.x / TPR : 0);
+        if (row >= rows) continue;
+        f32x4 xv[NV], zv[NV], gv[NV];
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * TPR + l) * 4, n = cg - c;
+            xv[i] = load4n<T, VEC>(x + row * x_ld + base + c, n);
+            zv[i] = load4n<T, VEC>(z + row * z_ld + base + c, n);
+            gv[i] = load4n<T, VEC>(dy + row * dy_ld + base + c, n);
+            const f32x4 wv = w ? load4n<float, VEC>(w + base + c, n) : one;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float gt = zv[i][j] * sigm(zv[i][j]);
+                const float v = j < n ? (FIRST ? xv[i][j] : xv[i][j] * gt) : 0.f;
+                const float g = FIRST ? gv[i][j] * wv[j] * gt : gv[i][j] * wv[j];
+                s1 = fmaf(v, v, s1);
+                s2 = fmaf(g, v, s2);
+            }
+        }
+        row_sum2<TPR>(s1, s2, s);
+        const float rstd = 1.f / sqrtf(s1 * inv + eps), m = s2 * inv * rstd;   // mean(g hat)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * TPR + l) * 4, n = cg - c;
+            const f32x4 wv = w ? load4n<float, VEC>(w + base + c, n) : one;
+            f32x4 ox, oz;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float slope;
+                const float gt = gate_of(zv[i][j], slope);
+                const float hat = (FIRST ? xv[i][j] : xv[i][j] * gt) * rstd;
+                const float g = FIRST ? gv[i][j] * wv[j] * gt : gv[i][j] * wv[j];
+                const float dv = rstd * fmaf(-hat, m, g);
+                ox[j] = FIRST ? dv : dv * gt;
+                oz[j] = FIRST ? gv[i][j] * hat * wv[j] * slope : dv * xv[i][j] * slope;
+                if (j < n) aw[i][j] = fmaf(gv[i][j], FIRST ? hat * gt : hat, aw[i][j]);
+            }
+            const int64_t at = row * C + base + c;
+            if (dx) store4n<T, VEC>(dx + at, ox, n);
+            if (dz) store4n<T, VEC>(dz + at, oz, n);
+        }
+    }
+    if (part) put_columns<TPR, NV>(aw, part + (int64_t)blockIdx.x * C + base, cg, cols);
+}
+
+bool gated_args(const char* who, int dtype, int64_t R, int C, int groups) {
+    if (!aas_dt_ok(dtype)) { aas_set_error("%s: dtype %d", who, dtype); return false; }
+    if (R < 0 || C < 1 || groups < 1 || C % groups) { aas_set_error("%s: R = %lld, C = %d, groups = %d", who, (long long)R, C, groups); return false; }
+    if (C / groups > NORM_MAX_C) { aas_set_error("%s: %d channels a group, at most %d", who, C / groups, NORM_MAX_C); return false; }
+    if (groups > 65535 || R * groups > 0x7fffffff) { aas_set_error("%s: R = %lld, groups = %d too large", who, (long long)R, groups); return false; }
+    return true;
+}
+
+}  // namespace
+
+extern "C" int aas_gated_norm_fwd(aasStream_t stream, int dtype, int64_t R, int C, int groups, const void* x, int64_t x_ld, const void* gate,
+                                  int64_t gate_ld, const float* weight, float eps, int norm_first, void* y) {
+    const char* who = "aas_gated_norm_fwd";
+    if (!gated_args(who, dtype, R, C, groups)) return 1;
+    if (R == 0) return 0;
+    AAS_CHECK(x && gate && y, "%s: null pointer", who);
+    const int es = aas_dt_size(dtype), cg = C / groups;
+    const bool vec = cg % 4 == 0 && x_ld % 4 == 0 && gate_ld % 4 == 0 && aas_aligned(x, 4 * es) && aas_aligned(gate, 4 * es) && aas_aligned(y, 4 * es) &&
+                     aas_aligned(weight, 16);
+    const unsigned grid = (unsigned)(cg <= 1024 ? (R * groups + 3) / 4 : R * groups);
+#define GO1(TPR, NV, VEC, FIRST)                                                                                                                  \
+    AAS_DT_SWITCH(dtype, E, hipLaunchKernelGGL((gated_fwd_kernel<E, TPR, NV, VEC, FIRST>), dim3(grid), dim3(TPR > 256 ? TPR : 256), 0,           \
+                                               (hipStream_t)stream, R, C, cg, groups, (const E*)x, x_ld, (const E*)gate, gate_ld, weight, eps, (E*)y))
+#define GO(TPR, NV, VEC) if (norm_first) { GO1(TPR, NV, VEC, true) } else { GO1(TPR, NV, VEC, false) }
+    AAS_ROW_SWITCH(cg, vec, GO);
+#undef GO
+#undef GO1
+    AAS_LAUNCH_CHECK(who);
+    return 0;
+}
+
+static int gated_blocks(int64_t R, int C, int groups) {              // workgroups per group: about 1024 in all
+    const int b = norm_bwd_blocks(R, C / groups), most = groups >= 1024 ? 1 : 1024 / groups;
+    return b < most ? b : most;
+}
+
+extern "C" size_t aas_gated_norm_bwd_ws_bytes(int64_t R, int C, int groups) {
+    if (R <= 0 || C <= 0 || groups <= 0 || C % groups) return 0;
+    return (size_t)gated_blocks(R, C, groups) * C * sizeof(float);
+}
+
+extern "C" int aas_gated_norm_bwd(aasStream_t stream, int dtype, int64_t R, int C, int groups, const void* dy, int64_t dy_ld, const void* x, int64_t x_ld,
+                                  const void* gate, int64_t gate_ld, const float* weight, float eps, int norm_first, void* dx, void* dgate,
+                                  float* dweight, void* ws) {
+    const char* who = "aas_gated_norm_bwd";
+    if (!gated_args(who, dtype, R, C, groups)) return 1;
+    hipStream_t s = (hipStream_t)stream;
+    int P = 0;
+    if (R > 0) {
+        AAS_CHECK(dy && x && gate && (ws || !dweight), "%s: null pointer", who);
+        const int es = aas_dt_size(dtype), cg = C / groups;
+        const bool vec = cg % 4 == 0 && dy_ld % 4 == 0 && x_ld % 4 == 0 && gate_ld % 4 == 0 && aas_aligned(dy, 4 * es) && aas_aligned(x, 4 * es) &&
+                         aas_aligned(gate, 4 * es) && aas_aligned(dx, 4 * es) && aas_aligned(dgate, 4 * es) && aas_aligned(weight, 16);
+        P = gated_blocks(R, C, groups);
+        float* part = dweight ? (float*)ws : nullptr;
+#define GO1(TPR, NV, VEC, FIRST)                                                                                                                       \
+    AAS_DT_SWITCH(dtype, E, hipLaunchKernelGGL((gated_bwd_kernel<E, TPR, NV, VEC, FIRST>), dim3(P, groups), dim3(TPR > 256 ? TPR : 256), 0, s, R, C,  \
+                                               cg, (const E*)dy, dy_ld, (const E*)x, x_ld, (const E*)gate, gate_ld, weight, eps, (E*)dx, (E*)dgate, part))
+#define GO(TPR, NV, VEC) if (norm_first) { GO1(TPR, NV, VEC, true) } else { GO1(TPR, NV, VEC, false) }
+        AAS_ROW_SWITCH(cg, vec, GO);
+#undef GO
+#undef GO1
+        AAS_LAUNCH_CHECK(who);
+    }
+    if (!dweight) return 0;
+    ColMap map = {{dweight, nullptr, nullptr, nullptr}, {C, 0, 0, 0}, 0, 1};
+    return aas_sum_partials(s, (const float*)ws, P, C, map, who);
+}

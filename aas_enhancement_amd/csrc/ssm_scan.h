@@ -1,0 +1,98 @@
+// Shared by the kernels of the selective state space scan (ssm_scan_fwd.hip, ssm_scan_bwd.hip).
+//
+//   d = softplus(dt + dt_bias),  h_s[t] = exp(d A_s) h_s[t-1] + d x B_s[t],  o = sum_s C_s h_s + D x,  y = o z sigmoid(z).
+//
+// Layout of a workgroup: 64 channels of one row n x 4 lanes a channel, each lane with NG groups of 4 states (state g*16 + 4*q + j for lane
+// q of the quad), so up to 16 NG states; the sum over a channel's states is two quad exchanges.  The time axis goes by in tiles of 16
+// frames staged in LDS: each thread loads four neighbouring channels of one frame and forms what depends on (frame, channel) only -
+// softplus, gates - ONCE, not once per state; B and C of the tile are read as quads by all channels.
+#pragma once
+#include "seq_common.h"
+
+constexpr int SCAN_CH = 64;      // channels per workgroup
+constexpr int SCAN_TT = 16;      // frames per tile
+constexpr int SCAN_YP = 80;      // pitch of a [16 frames][64 channels] tile that the scanning lanes write: 4 frames x 16 channels a wave, no two on one bank
+constexpr float SCAN_LOG2E = 1.4426950408889634f;
+constexpr float SCAN_LN2 = 0.6931471805599453f;
+
+struct ScanDev {                 // aasScan with the pointers' types left to the kernels, plus what the host derives
+    int T, N, Ch, S, G, softplus;
+    int cpg, nbg;                // channels per group, workgroups per group
+    int tiles_per_chunk, nchunk; // chunks of the time axis (1: none)
+    int svec;                    // rows of S fp32 states (A, the state) can be read four at a time
+    const void *x, *dt, *z, *B, *C;
+    const float *A, *D, *dt_bias;
+    const int* len;
+    int64_t x_st, x_sn, dt_st, dt_sn, z_st, z_sn, B_st, B_sn, B_sg, C_st, C_sn, C_sg;
+};
+
+struct ScanBlock {               // where a workgroup stands
+    int n, grp, c0, cn;          // row, group of B / C, first channel, channels (<= 64)
+};
+__device__ __forceinline__ ScanBlock scan_block(const ScanDev& a) {
+    ScanBlock b;
+    const int per_n = a.nbg * a.G;
+    b.n = blockIdx.x / per_n;
+    const int cb = blockIdx.x - b.n * per_n;
+    b.grp = cb / a.nbg;
+    const int i = cb - b.grp * a.nbg;
+    b.c0 = b.grp * a.cpg + i * SCAN_CH;
+    const int left = a.cpg - i * SCAN_CH;
+    b.cn = left < SCAN_CH ? left : SCAN_CH;
+    return b;
+}
+
+// log(1 + e^-|v|) + max(v, 0), with e = e^-|v| also handed back.  log(1 + e) = 2 atanh(e / (2 + e)) as its series: e <= 1, so the argument
+// is at most 1/3 and nine terms leave 3^-20 / 19 of the sum - full relative accuracy also where e is tiny (d of 1e-3 and below), which
+// log2(1 + e) in fp32 has not.
+__device__ __forceinline__ float softplusf_(float v, float* e_out) {
+    const float e = expf(-fabsf(v));
+    *e_out = e;
+    const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
+    float p = 1.f / 17.f;
+    p = fmaf(p, q, 1.f / 15.f);
+    p = fmaf(p, q, 1.f / 13.f);
+    p = fmaf(p, q, 1.f / 11.f);
+    p = fmaf(p, q, 1.f / 9.f);
+    p = fmaf(p, q, 1.f / 7.f);
+    p = fmaf(p, q, 1.f / 5.f);
+    p = fmaf(p, q, 1.f / 3.f);
+    p = fmaf(p, q, 1.f);
+    return fmaf(2.f * s, p, fmaxf(v, 0.f));
+}
+// d and, for the backward pass, its derivative
+__device__ __forceinline__ float scan_delta(float dt, float bias, int softplus) {
+    const float v = dt + bias;
+    if (!softplus) return v;
+    float e;
+    const float d = softplusf_(v, &e);
+    return v != v ? v : d;                              // (fmaxf would drop a NaN)
+}
+__device__ __forceinline__ float scan_delta_grad(float dt, float bias, int softplus) {
+    if (!softplus) return 1.f;
+    return sigm(dt + bias);
+}
+
+// the 4 states of lane q, group g, of a [S] row (zeros behind the last)
+__device__ __forceinline__ f32x4 scan_states4(const float* row, int s0, int S, bool vec) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (vec) { if (s0 < S) v = *reinterpret_cast<const f32x4*>(row + s0); }
+    else
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (s0 + j < S) v[j] = row[s0 + j];
+    return v;
+}
+__device__ __forceinline__ void scan_put_states4(float* row, int s0, int S, bool vec, f32x4 v) {
+    if (vec) { if (s0 < S) *reinterpret_cast<f32x4*>(row + s0) = v; }
+    else
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (s0 + j < S) row[s0 + j] = v[j];
+}
+
+// host side
+int scan_check(const char* who, const aasScan* d);             // 0 fine, 1 error (aas_last_error)
+void scan_dev(const aasScan* d, ScanDev* a);                   // fills everything but the chunks
+bool scan_vec(const ScanDev& a, int dtype);                    // rows of x, dt, z can be read four channels at a time
+static inline int scan_tiles(int T) { return cdiv(T, SCAN_TT); }

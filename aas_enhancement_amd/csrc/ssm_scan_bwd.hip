@@ -1,0 +1,331 @@
+// Selective state space scan, backward (ssm_scan.h has the layout).  With go = dy z sigmoid(z) and g_s[t] the gradient of h_s[t]:
+//
+//   g_s[t] = C_s go + a_s[t+1] g_s[t+1],  a_s = exp(d A_s),     p_s = a_s h_s[t-1],  q_s = g_s p_s,
+//   u = sum_s g_s B_s,  w = sum_s q_s A_s:   dx = D go + d u,   dd = w + x u,   ddt = dd softplus',   dz = dy o (z sigmoid(z))',
+//   dA_s = sum_{t,n} q_s d,   dB_s = sum_c g_s d x,   dC_s = sum_c go h_s,   dD = sum go x,   ddt_bias = sum ddt.
+//
+// Tiles of 16 frames from the last to the first: a lane runs forward from the state that the forward pass kept in front of the tile,
+// holding p of the 16 frames in registers, then back through them.  dB and dC are sums over channels: eight values a lane (four
+// states x {dB, dC}) over the 16 channels of a wave go by exchanges that halve the number of values with the number of lanes still to
+// add (lane halves, rows of 16, then within the row), then over the four waves through LDS, then - plain stores, no atomics - over the
+// workgroups by a second launch.
+#include "ssm_scan.h"
+
+namespace {
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float add_halves(float a, float b) {         // lanes 0-31: a summed over the halves; lanes 32-63: b
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float add_rows(float a, float b) {           // rows 0, 2 of 16 lanes: a summed over row pairs; rows 1, 3: b
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+template <int CTRL> __device__ __forceinline__ float add_dpp(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+constexpr int ROW_ROR_4 = 0x124, ROW_ROR_8 = 0x128;
+
+// v[0..7] summed over the 16 channels of the wave (lane bits 2 .. 5); the lane is left with the sum of value
+// (bit 5) + 2 (bit 4) + 4 (bit 3) of its lane number
+__device__ __forceinline__ float sum_channels8(const float v[8], bool bit3) {
+    const float a = add_rows(add_halves(v[0], v[1]), add_halves(v[2], v[3]));
+    const float b = add_rows(add_halves(v[4], v[5]), add_halves(v[6], v[7]));
+    const float a1 = add_dpp<ROW_ROR_4>(add_dpp<ROW_ROR_8>(a)), b1 = add_dpp<ROW_ROR_4>(add_dpp<ROW_ROR_8>(b));
+    return bit3 ? b1 : a1;
+}
+
+template <class T, int NG, bool VEC>
+__global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __restrict__ dy, int64_t dy_st, int64_t dy_sn, const float* __restrict__ hsave,
+                                                       T* __restrict__ dx, T* __restrict__ ddt, T* __restrict__ dz, float* __restrict__ part_bc,
+                                                       float* __restrict__ part_a, float* __restrict__ part_d) {
+    __shared__ float2 dd[SCAN_TT][SCAN_CH];             // d, d x
+    __shared__ float go[SCAN_TT][SCAN_CH];
+    __shared__ __align__(16) float bs[SCAN_TT][NG * 16], cs[SCAN_TT][NG * 16];
+    __shared__ float us[SCAN_TT][SCAN_YP], ws[SCAN_TT][SCAN_YP], os[SCAN_TT][SCAN_YP];
+    __shared__ float bc[4][SCAN_TT][NG * 32];           // per wave, frame: dB of the 16 NG states, dC
+    const ScanBlock b = scan_block(a);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = tid & 3, cw = tid >> 2;
+    const int lr = tid >> 4, lc = (tid & 15) * 4, ln = b.cn - lc;
+    const int L = row_length(a.len, b.n, a.T);
+    const bool on = cw < b.cn, svec = a.svec != 0;
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    const T* xp = (const T*)a.x + b.n * a.x_sn + b.c0 + lc;
+    const T* tp = (const T*)a.dt + b.n * a.dt_sn + b.c0 + lc;
+    const T* zp = a.z ? (const T*)a.z + b.n * a.z_sn + b.c0 + lc : nullptr;
+    const T* gp = dy + b.n * dy_sn + b.c0 + lc;
+    const T* bp = (const T*)a.B + b.n * a.B_sn + b.grp * a.B_sg;
+    const T* cp = (const T*)a.C + b.n * a.C_sn + b.grp * a.C_sg;
+    const int64_t srow = ((int64_t)b.n * a.Ch + b.c0 + cw) * a.S;
+
+    f32x4 A2[NG], dA[NG], carry[NG];                                    // carry = a[t+1] g[t+1]
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        A2[g] = on ? scan_states4(a.A + (int64_t)(b.c0 + cw) * a.S, g * 16 + 4 * q, a.S, svec) * SCAN_LOG2E : zero;
+        dA[g] = carry[g] = zero;
+    }
+    const f32x4 bias = a.dt_bias ? load4n<float, false>(a.dt_bias + b.c0 + lc, ln) : zero;
+    const f32x4 Dv = a.D ? load4n<float, false>(a.D + b.c0 + lc, ln) : zero;
+    f32x4 dD = zero, dbias = zero;
+
+    f32x4 xr, tr, zr = zero, gr, h0[NG];
+    float br[NG], cr[NG];
+    auto load = [&](int tile) {
+        const int64_t t = (int64_t)tile * SCAN_TT + lr;
+        const int m = t < L ? ln : 0;
+        xr = load4n<T, VEC>(xp + t * a.x_st, m);
+        tr = load4n<T, VEC>(tp + t * a.dt_st, m);
+        if (zp) zr = load4n<T, VEC>(zp + t * a.z_st, m);
+        gr = load4n<T, VEC>(gp + t * dy_st, m);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const int s = g * 16 + (tid & 15);
+            const bool in = t < L && s < a.S;
+            br[g] = in ? (float)bp[t * a.B_st + s] : 0.f;
+            cr[g] = in ? (float)cp[t * a.C_st + s] : 0.f;
+            h0[g] = on ? scan_states4(hsave + ((int64_t)tile * a.N * a.Ch) * a.S + srow, g * 16 + 4 * q, a.S, svec) : zero;
+        }
+    };
+    const int tiles = (L + SCAN_TT - 1) / SCAN_TT;
+    const int64_t orow = (int64_t)a.N * a.Ch, obase = (int64_t)b.n * a.Ch + b.c0 + lc;
+    const int nblk = a.nbg;
+    const int cb = (b.c0 - b.grp * a.cpg) / SCAN_CH;
+    if (tiles > 0) load(tiles - 1);
+    for (int k = tiles - 1; k >= 0; --k) {
+        const int64_t t = (int64_t)k * SCAN_TT + lr;
+        const bool live = t < L;
+        const f32x4 xe = xr, te = tr, ze = zr, ge = gr;
+        f32x4 de, oe;                                                   // d, go of this thread's elements
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            de[i] = live && i < ln ? scan_delta(te[i], bias[i], a.softplus) : 0.f;
+            oe[i] = zp ? ge[i] * (ze[i] * sigm(ze[i])) : ge[i];
+            dd[lr][lc + i] = make_float2(de[i], de[i] * xe[i]);
+            go[lr][lc + i] = oe[i];
+        }
+        f32x4 h[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            bs[lr][g * 16 + (tid & 15)] = br[g];
+            cs[lr][g * 16 + (tid & 15)] = cr[g];
+            h[g] = h0[g];
+        }
+        if (k > 0) load(k - 1);
+        __syncthreads();
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            f32x4 p[SCAN_TT];                                           // a h[t-1]
+            float keep = 0.f;
+#pragma unroll
+            for (int i = 0; i < SCAN_TT; ++i) {
+                const float2 d = dd[i][cw];
+                const f32x4 B = reinterpret_cast<const f32x4*>(bs[i])[g * 4 + q];
+                float acc = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    p[i][j] = __builtin_amdgcn_exp2f(d.x * A2[g][j]) * h[g][j];
+                    h[g][j] = fmaf(d.y, B[j], p[i][j]);
+                }
+                const f32x4 C = reinterpret_cast<const f32x4*>(cs[i])[g * 4 + q];     // (o, wanted for dz; without z it costs a few per cent)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc = fmaf(h[g][j], C[j], acc);
+                acc = quad_sum(acc);
+                keep = q == (i & 3) ? acc : keep;
+                if ((i & 3) == 3) {
+                    float* o = &os[(i & ~3) + q][cw];
+                    *o = g == 0 ? keep : *o + keep;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // B, d and the exponentials are read and formed again (an address the compiler cannot match with the one above): kept from the
+            // forward run, they would be 160 registers
+            int ch = cw, sq = g * 4 + q;
+            asm volatile("" : "+v"(ch), "+v"(sq));
+            float ku = 0.f, kw = 0.f;
+#pragma unroll
+            for (int i = SCAN_TT - 1; i >= 0; --i) {
+                const float2 d = dd[i][ch];
+                const float o = go[i][ch];
+                const f32x4 B = reinterpret_cast<const f32x4*>(bs[i])[sq];
+                const f32x4 C = reinterpret_cast<const f32x4*>(cs[i])[sq];
+                float u = 0.f, w = 0.f, v[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float gh = fmaf(C[j], o, carry[g][j]);
+                    v[4 + j] = o * fmaf(d.y, B[j], p[i][j]);
+                    v[j] = gh * d.y;
+                    u = fmaf(gh, B[j], u);
+                    const float r = gh * p[i][j];
+                    w = fmaf(r, A2[g][j], w);
+                    dA[g][j] = fmaf(r, d.x, dA[g][j]);
+                    carry[g][j] = gh * __builtin_amdgcn_exp2f(d.x * A2[g][j]);
+                }
+                u = quad_sum(u);
+                w = quad_sum(w);
+                ku = q == (i & 3) ? u : ku;
+                kw = q == (i & 3) ? w : kw;
+                if ((i & 3) == 0) {
+                    float *pu = &us[i + q][cw], *pw = &ws[i + q][cw];
+                    *pu = g == 0 ? ku : *pu + ku;
+                    *pw = g == 0 ? kw : *pw + kw;
+                }
+                asm volatile("" : "+v"(dA[g][0]), "+v"(dA[g][1]), "+v"(dA[g][2]), "+v"(dA[g][3]));   // added up here, not 64 products kept for later
+                const float s = sum_channels8(v, (lane & 8) != 0);
+                __builtin_amdgcn_sched_barrier(0);
+                // value (bit 5) + 2 (bit 4) is the state of the quad, bit 3 says dB or dC; the lanes that differ in bit 2 hold the same
+                bc[wave][i][((lane & 8) ? NG * 16 : 0) + g * 16 + 4 * q + ((lane >> 5) & 1) + ((lane >> 3) & 2)] = s;
+            }
+        }
+        __syncthreads();
+        if (t < a.T) {
+            f32x4 vx, vt, vz;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float u = us[lr][lc + i];
+                vx[i] = fmaf(de[i], u, Dv[i] * oe[i]);
+                vt[i] = fmaf(ws[lr][lc + i], SCAN_LN2, xe[i] * u) * scan_delta_grad(te[i], bias[i], a.softplus);
+                if (zp) {
+                    const float s = sigm(ze[i]), o = fmaf(Dv[i], xe[i], os[lr][lc + i]);
+                    vz[i] = ge[i] * o * s * fmaf(ze[i], 1.f - s, 1.f);
+                }
+                if (live && i < ln) {
+                    dD[i] = fmaf(oe[i], xe[i], dD[i]);
+                    dbias[i] += vt[i];
+                } else {
+                    vx[i] = vt[i] = vz[i] = 0.f;
+                }
+            }
+            const int64_t at = t * orow + obase;
+            store4n<T, VEC>(dx + at, vx, ln);
+            store4n<T, VEC>(ddt + at, vt, ln);
+            if (dz) store4n<T, VEC>(dz + at, vz, ln);
+        }
+        // partial dB, dC of this workgroup: [T][N][G][nblk][2][S]
+#pragma unroll
+        for (int i = 0; i < 2 * NG; ++i) {
+            const int e = tid + 256 * i, f = e / (NG * 32), j = e - f * (NG * 32);
+            const int which = j >= NG * 16 ? 1 : 0, s = j - which * NG * 16;
+            const int64_t tt = (int64_t)k * SCAN_TT + f;
+            if (s < a.S && tt < L)
+                part_bc[((((tt * a.N + b.n) * a.G + b.grp) * nblk + cb) * 2 + which) * a.S + s] =
+                    (bc[0][f][j] + bc[1][f][j]) + (bc[2][f][j] + bc[3][f][j]);
+        }
+    }
+    for (int64_t t = (int64_t)tiles * SCAN_TT + lr; t < a.T; t += SCAN_TT) {
+        const int64_t at = t * orow + obase;
+        store4n<T, VEC>(dx + at, zero, ln);
+        store4n<T, VEC>(ddt + at, zero, ln);
+        if (dz) store4n<T, VEC>(dz + at, zero, ln);
+    }
+    if (on)
+#pragma unroll
+        for (int g = 0; g < NG; ++g) scan_put_states4(part_a + srow, g * 16 + 4 * q, a.S, svec, dA[g]);
+    __syncthreads();                                                    // (the last tile's readers of us, ws)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        us[lr][lc + i] = dD[i];
+        ws[lr][lc + i] = dbias[i];
+    }
+    __syncthreads();
+    if (tid < 2 * SCAN_CH) {
+        const int c = tid & (SCAN_CH - 1);
+        const float(*from)[SCAN_YP] = tid < SCAN_CH ? us : ws;
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < SCAN_TT; ++i) v += from[i][c];
+        if (c < b.cn) part_d[((int64_t)b.n * 2 + (tid >= SCAN_CH ? 1 : 0)) * a.Ch + b.c0 + c] = v;
+    }
+}
+
+// dB, dC [T,N,G,S] from the partial sums of the group's workgroups, frames behind a row's end zero
+template <class T>
+__global__ __launch_bounds__(256) void scan_bc_kernel(const float* __restrict__ part, int TT, int N, int G, int S, int nblk, const int* __restrict__ len,
+                                                      T* __restrict__ dB, T* __restrict__ dC) {
+    const int64_t total = (int64_t)TT * N * G * S;
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
+        const int64_t row = e / S;
+        const int s = (int)(e - row * S);
+        const int64_t tn = row / G;
+        const int n = (int)(tn % N);
+        float vb = 0.f, vc = 0.f;
+        if (tn / N < row_length(len, n, TT)) {
+            const float* p = part + row * nblk * 2 * S + s;
+            for (int i = 0; i < nblk; ++i) { vb += p[(int64_t)(2 * i) * S]; vc += p[(int64_t)(2 * i + 1) * S]; }
+        }
+        dB[e] = (T)vb;
+        dC[e] = (T)vc;
+    }
+}
+
+struct BwdWs { size_t bc, a, d, total; };               // byte offsets
+BwdWs bwd_ws(int T, int N, int Ch, int S, int G) {
+    BwdWs w;
+    auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+    w.bc = 0;
+    w.a = up((size_t)T * N * G * cdiv(Ch / G, SCAN_CH) * 2 * S * sizeof(float));
+    w.d = w.a + up((size_t)N * Ch * S * sizeof(float));
+    w.total = w.d + up((size_t)N * 2 * Ch * sizeof(float));
+    return w;
+}
+
+template <class T>
+void launch_bwd(hipStream_t s, const ScanDev& a, bool vec, const void* dy, int64_t dy_st, int64_t dy_sn, const float* hsave, void* dx, void* ddt, void* dz,
+                float* bc, float* pa, float* pd) {
+    const dim3 grid((unsigned)((int64_t)a.N * a.nbg * a.G));
+#define AAS_GO(NG_)                                                                                                                   \
+    do {                                                                                                                              \
+        if (vec)                                                                                                                      \
+            hipLaunchKernelGGL((scan_bwd_kernel<T, NG_, true>), grid, dim3(256), 0, s, a, (const T*)dy, dy_st, dy_sn, hsave, (T*)dx,  \
+                               (T*)ddt, (T*)dz, bc, pa, pd);                                                                          \
+        else                                                                                                                          \
+            hipLaunchKernelGGL((scan_bwd_kernel<T, NG_, false>), grid, dim3(256), 0, s, a, (const T*)dy, dy_st, dy_sn, hsave, (T*)dx, \
+                               (T*)ddt, (T*)dz, bc, pa, pd);                                                                          \
+    } while (0)
+    if (a.S <= 16) AAS_GO(1);
+    else if (a.S <= 32) AAS_GO(2);
+    else AAS_GO(4);
+#undef AAS_GO
+}
+
+}  // namespace
+
+extern "C" size_t aas_ssm_scan_bwd_ws_bytes(int T, int N, int Ch, int S, int G) {
+    if (T <= 0 || N <= 0 || Ch <= 0 || S <= 0 || G <= 0 || Ch % G) return 0;
+    return bwd_ws(T, N, Ch, S, G).total;
+}
+
+extern "C" int aas_ssm_scan_bwd(aasStream_t stream, const aasScan* d, const void* dy, int64_t dy_st, int64_t dy_sn, const float* hsave, void* dx,
+                                void* ddt, void* dz, void* dB, void* dC, float* dA, float* dD, float* ddt_bias, void* ws) {
+    const char* who = "aas_ssm_scan_bwd";
+    if (scan_check(who, d)) return 1;
+    hipStream_t s = (hipStream_t)stream;
+    const bool empty = d->T == 0 || d->N == 0;
+    if (d->Ch == 0) return 0;
+    AAS_CHECK(dA != nullptr, "%s: null pointer", who);
+    const BwdWs w = empty ? BwdWs{0, 0, 0, 0} : bwd_ws(d->T, d->N, d->Ch, d->S, d->G);
+    char* base = (char*)ws;
+    if (!empty) {
+        AAS_CHECK(dy && hsave && dx && ddt && dB && dC && ws && (dz || !d->z), "%s: null pointer", who);
+        AAS_CHECK(aas_aligned(hsave, 16) && aas_aligned(ws, 16), "%s: hsave and ws must be 16-byte aligned", who);
+        ScanDev a;
+        scan_dev(d, &a);
+        const int al = 4 * aas_dt_size(d->dtype);
+        const bool vec = scan_vec(a, d->dtype) && dy_st % 4 == 0 && dy_sn % 4 == 0 && aas_aligned(dy, al) && aas_aligned(dx, al) && aas_aligned(ddt, al) &&
+                         (!dz || aas_aligned(dz, al));
+        AAS_DT_SWITCH(d->dtype, E, launch_bwd<E>(s, a, vec, dy, dy_st, dy_sn, hsave, dx, ddt, d->z ? dz : nullptr, (float*)(base + w.bc),
+                                                 (float*)(base + w.a), (float*)(base + w.d)));
+        AAS_LAUNCH_CHECK(who);
+        const int64_t total = (int64_t)d->T * d->N * d->G * d->S;
+        const int blocks = (int)(total / 256 + 1 < 4096 ? total / 256 + 1 : 4096);
+        AAS_DT_SWITCH(d->dtype, E, hipLaunchKernelGGL(scan_bc_kernel<E>, dim3(blocks), dim3(256), 0, s, (const float*)(base + w.bc), d->T, d->N, d->G,
+                                                      d->S, a.nbg, d->len, (E*)dB, (E*)dC));
+        AAS_LAUNCH_CHECK(who);
+    }
+    const int P = empty ? 0 : d->N;
+    ColMap ma = {{dA, nullptr, nullptr, nullptr}, {d->Ch * d->S, 0, 0, 0}, 0, 1};
+    if (aas_sum_partials(s, (const float*)(base + w.a), P, d->Ch * d->S, ma, who)) return 2;
+    if (!dD && !ddt_bias) return 0;
+    ColMap md = {{dD, ddt_bias, nullptr, nullptr}, {d->Ch, d->Ch, 0, 0}, 0, 2};
+    return aas_sum_partials(s, (const float*)(base + w.d), P, 2 * d->Ch, md, who);
+}

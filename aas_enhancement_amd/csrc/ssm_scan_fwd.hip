@@ -1,0 +1,196 @@
+// Selective state space scan, forward (ssm_scan.h has the mathematics and the layout).
+#include "ssm_scan.h"
+
+namespace {
+
+template <class T, int NG, bool VEC>
+__global__ __launch_bounds__(256) void scan_fwd_kernel(ScanDev a, float* __restrict__ state, T* __restrict__ y, float* __restrict__ hsave) {
+    __shared__ float2 dd[2][SCAN_TT][SCAN_CH];          // d, d x
+    __shared__ __align__(16) float bs[2][SCAN_TT][NG * 16], cs[2][SCAN_TT][NG * 16];
+    __shared__ float ys[2][SCAN_TT][SCAN_YP];
+    const ScanBlock b = scan_block(a);
+    const int tid = threadIdx.x, q = tid & 3, cw = tid >> 2;            // scanning: lane q of channel cw
+    const int lr = tid >> 4, lc = (tid & 15) * 4, ln = b.cn - lc;       // loading: channels lc .. lc+3 of frame lr of the tile
+    const int L = row_length(a.len, b.n, a.T);
+    const bool on = cw < b.cn, svec = a.svec != 0;
+    const T* xp = (const T*)a.x + b.n * a.x_sn + b.c0 + lc;
+    const T* tp = (const T*)a.dt + b.n * a.dt_sn + b.c0 + lc;
+    const T* zp = a.z ? (const T*)a.z + b.n * a.z_sn + b.c0 + lc : nullptr;
+    const T* bp = (const T*)a.B + b.n * a.B_sn + b.grp * a.B_sg;
+    const T* cp = (const T*)a.C + b.n * a.C_sn + b.grp * a.C_sg;
+
+    f32x4 A2[NG], h[NG];                                                // A log2(e): exp(d A) is one exp2
+    const int64_t srow = ((int64_t)b.n * a.Ch + b.c0 + cw) * a.S;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        const int s0 = g * 16 + 4 * q;
+        A2[g] = h[g] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (on) {
+            A2[g] = scan_states4(a.A + (int64_t)(b.c0 + cw) * a.S, s0, a.S, svec) * SCAN_LOG2E;
+            if (state) h[g] = scan_states4(state + srow, s0, a.S, svec);
+        }
+    }
+    const f32x4 bias = a.dt_bias ? load4n<float, false>(a.dt_bias + b.c0 + lc, ln) : f32x4{0.f, 0.f, 0.f, 0.f};
+    const f32x4 Dv = a.D ? load4n<float, false>(a.D + b.c0 + lc, ln) : f32x4{0.f, 0.f, 0.f, 0.f};
+
+    f32x4 xr, tr, zr, xe, ze;
+    float br[NG], cr[NG];
+    auto load = [&](int tile) {
+        const int64_t t = (int64_t)tile * SCAN_TT + lr;
+        const int m = t < L ? ln : 0;
+        xr = load4n<T, VEC>(xp + t * a.x_st, m);
+        tr = load4n<T, VEC>(tp + t * a.dt_st, m);
+        if (zp) zr = load4n<T, VEC>(zp + t * a.z_st, m);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {                                  // one state of one frame per thread and group
+            const int s = g * 16 + (tid & 15);
+            const bool in = t < L && s < a.S;
+            br[g] = in ? (float)bp[t * a.B_st + s] : 0.f;
+            cr[g] = in ? (float)cp[t * a.C_st + s] : 0.f;
+        }
+    };
+    auto stage = [&](int tile, int u) {
+        const bool live = tile * SCAN_TT + lr < L;                      // behind the row's end: d = 0 leaves the state as it is
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float d = live && i < ln ? scan_delta(tr[i], bias[i], a.softplus) : 0.f;
+            dd[u][lr][lc + i] = make_float2(d, d * xr[i]);
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            bs[u][lr][g * 16 + (tid & 15)] = br[g];
+            cs[u][lr][g * 16 + (tid & 15)] = cr[g];
+        }
+    };
+    const int tiles = (L + SCAN_TT - 1) / SCAN_TT;
+    T* yp = y + ((int64_t)lr * a.N + b.n) * a.Ch + b.c0 + lc;
+    const int64_t ytile = (int64_t)SCAN_TT * a.N * a.Ch;
+    if (tiles > 0) {
+        load(0);
+        stage(0, 0);
+        xe = xr;
+        ze = zr;
+        if (tiles > 1) load(1);
+        __syncthreads();
+    }
+    for (int k = 0; k < tiles; ++k, yp += ytile) {
+        const int u = k & 1;
+        if (hsave && on) {
+            float* hp = hsave + ((int64_t)k * a.N * a.Ch) * a.S + srow;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) scan_put_states4(hp, g * 16 + 4 * q, a.S, svec, h[g]);
+        }
+#pragma unroll 1
+        for (int t = 0; t < SCAN_TT; t += 4) {
+            float keep = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 d = dd[u][t + i][cw];
+                float acc = 0.f;
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const f32x4 B = reinterpret_cast<const f32x4*>(bs[u][t + i])[g * 4 + q];
+                    const f32x4 C = reinterpret_cast<const f32x4*>(cs[u][t + i])[g * 4 + q];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        h[g][j] = fmaf(__builtin_amdgcn_exp2f(d.x * A2[g][j]), h[g][j], d.y * B[j]);
+                        acc = fmaf(h[g][j], C[j], acc);
+                    }
+                }
+                acc = quad_sum(acc);
+                keep = q == i ? acc : keep;
+            }
+            ys[u][t + q][cw] = keep;
+        }
+        f32x4 xn = xr, zn = zr;
+        if (k + 1 < tiles) {
+            stage(k + 1, u ^ 1);
+            if (k + 2 < tiles) load(k + 2);
+        }
+        __syncthreads();
+        if (k * SCAN_TT + lr < a.T) {
+            f32x4 o;
+            const bool live = k * SCAN_TT + lr < L;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                o[i] = fmaf(Dv[i], xe[i], ys[u][lr][lc + i]);
+                if (zp) o[i] *= ze[i] * sigm(ze[i]);
+                if (!live) o[i] = 0.f;
+            }
+            store4n<T, VEC>(yp, o, ln);
+        }
+        xe = xn;
+        ze = zn;
+    }
+    for (int t = tiles * SCAN_TT + lr; t < a.T; t += SCAN_TT, yp += ytile) store4n<T, VEC>(yp, f32x4{0.f, 0.f, 0.f, 0.f}, ln);
+    if (state && on)
+#pragma unroll
+        for (int g = 0; g < NG; ++g) scan_put_states4(state + srow, g * 16 + 4 * q, a.S, svec, h[g]);
+}
+
+template <class T>
+void launch_fwd(hipStream_t s, const ScanDev& a, bool vec, float* state, void* y, float* hsave) {
+    const dim3 grid((unsigned)((int64_t)a.N * a.nbg * a.G));
+#define AAS_GO(NG_)                                                                                                                   \
+    do {                                                                                                                              \
+        if (vec) hipLaunchKernelGGL((scan_fwd_kernel<T, NG_, true>), grid, dim3(256), 0, s, a, state, (T*)y, hsave);                  \
+        else hipLaunchKernelGGL((scan_fwd_kernel<T, NG_, false>), grid, dim3(256), 0, s, a, state, (T*)y, hsave);                     \
+    } while (0)
+    if (a.S <= 16) AAS_GO(1);
+    else if (a.S <= 32) AAS_GO(2);
+    else AAS_GO(4);
+#undef AAS_GO
+}
+
+}  // namespace
+
+int scan_check(const char* who, const aasScan* d) {
+    AAS_CHECK(d != nullptr, "%s: null descriptor", who);
+    AAS_CHECK(d->size == (int)sizeof(aasScan), "%s: aasScan.size = %d, this library's is %d", who, d->size, (int)sizeof(aasScan));
+    AAS_CHECK(aas_dt_ok(d->dtype), "%s: dtype %d", who, d->dtype);
+    AAS_CHECK(d->T >= 0 && d->N >= 0 && d->Ch >= 0, "%s: T = %d, N = %d, Ch = %d", who, d->T, d->N, d->Ch);
+    AAS_CHECK(d->T <= 0x7fffffff - 2 * SCAN_TT, "%s: T = %d too long", who, d->T);
+    AAS_CHECK(d->S >= 1 && d->S <= 64, "%s: S = %d, must be 1 to 64", who, d->S);
+    AAS_CHECK(d->G >= 1 && d->Ch % d->G == 0, "%s: Ch = %d is no multiple of G = %d", who, d->Ch, d->G);
+    AAS_CHECK((int64_t)d->N * (cdiv(d->Ch / d->G, SCAN_CH) * (int64_t)d->G) <= 0x7fffffff, "%s: N = %d, Ch = %d too large", who, d->N, d->Ch);
+    if (d->T == 0 || d->N == 0 || d->Ch == 0) return 0;
+    AAS_CHECK(d->x && d->dt && d->A && d->B && d->C, "%s: null pointer", who);
+    return 0;
+}
+
+void scan_dev(const aasScan* d, ScanDev* a) {
+    a->T = d->T; a->N = d->N; a->Ch = d->Ch; a->S = d->S; a->G = d->G; a->softplus = d->softplus;
+    a->cpg = d->Ch / d->G;
+    a->nbg = cdiv(a->cpg, SCAN_CH);
+    a->tiles_per_chunk = scan_tiles(d->T);
+    a->nchunk = 1;
+    a->svec = d->S % 4 == 0 && aas_aligned(d->A, 16);
+    a->x = d->x; a->dt = d->dt; a->z = d->z; a->B = d->B; a->C = d->C;
+    a->A = d->A; a->D = d->D; a->dt_bias = d->dt_bias; a->len = d->len;
+    a->x_st = d->x_st; a->x_sn = d->x_sn; a->dt_st = d->dt_st; a->dt_sn = d->dt_sn; a->z_st = d->z_st; a->z_sn = d->z_sn;
+    a->B_st = d->B_st; a->B_sn = d->B_sn; a->B_sg = d->B_sg; a->C_st = d->C_st; a->C_sn = d->C_sn; a->C_sg = d->C_sg;
+}
+
+// four channels at a time: channels of a group and every stride a multiple of four, bases on four elements (svec says
+// the same of A and the states)
+bool scan_vec(const ScanDev& a, int dtype) {
+    const int al = 4 * aas_dt_size(dtype);
+    return a.Ch % 4 == 0 && a.cpg % 4 == 0 && a.x_st % 4 == 0 && a.x_sn % 4 == 0 && a.dt_st % 4 == 0 && a.dt_sn % 4 == 0 && aas_aligned(a.x, al) &&
+           aas_aligned(a.dt, al) && (!a.z || (a.z_st % 4 == 0 && a.z_sn % 4 == 0 && aas_aligned(a.z, al)));
+}
+
+extern "C" size_t aas_ssm_scan_fwd_ws_bytes(int T, int N, int Ch, int S, int G) { return 0; }
+
+extern "C" int aas_ssm_scan_fwd(aasStream_t stream, const aasScan* d, float* state, void* y, float* hsave, void* ws) {
+    if (scan_check("aas_ssm_scan_fwd", d)) return 1;
+    if (d->T == 0 || d->N == 0 || d->Ch == 0) return 0;
+    AAS_CHECK(y != nullptr, "aas_ssm_scan_fwd: null pointer");
+    AAS_CHECK(aas_aligned(hsave, 16), "aas_ssm_scan_fwd: hsave must be 16-byte aligned");
+    ScanDev a;
+    scan_dev(d, &a);
+    if (!aas_aligned(state, 16)) a.svec = 0;
+    const bool vec = scan_vec(a, d->dtype) && aas_aligned(y, 4 * aas_dt_size(d->dtype));
+    AAS_DT_SWITCH(d->dtype, E, launch_fwd<E>((hipStream_t)stream, a, vec, state, y, hsave));
+    AAS_LAUNCH_CHECK("aas_ssm_scan_fwd");
+    return 0;
+}

@@ -2283,3 +2283,7 @@ def adam_step(p, g, m, v, vmax, lr, beta1, beta2, eps, step, amsgrad=True, grad_
 def sgd_nesterov_step(p, g, buf, lr, momentum, grad_scale=1.0):
     check(lib().aas_sgd_nesterov_f32(stream(), ptr(p), ptr(g), ptr(buf), p.numel(), float(lr), float(momentum), float(grad_scale)),
           "aas_sgd_nesterov_f32")
+
+
+# ------------------------------------------------------------------------------------------------- causal sequence operators (ops_seq.py)
+from .ops_seq import causal_conv1d, dropout, dropout_counters, gated_norm, residual_norm, ssm_scan  # noqa: E402,F401

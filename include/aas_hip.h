@@ -532,6 +532,86 @@ int aas_lmfb320_fwd(aasStream_t stream, const float* wave, const int* d_lens, in
                     const void* tables, const float* window, const int* mel_start, const int* mel_cnt,
                     const float* mel_w, int mel_maxw, float* out);
 
+/* ---------------------------------------------------------------- causal sequence operators ---
+ * The parts of a causal residual block over time-major activations [T, N, C] - what a live (frame by frame) enhancer needs beside the
+ * bidirectional layers above, which read the whole utterance.  Types: `dtype` (AAS_DT_*) is that of the activations and of their
+ * gradients; parameters, their gradients, states, statistics and every sum are fp32.  Activation INPUTS are views: channel stride 1
+ * and element strides (time, row) or a row pitch of the caller's; outputs are contiguous.  `len` (device int32 [N], may be NULL): frames
+ * of each row of a padded batch, brought into [0, T]; frames behind a row's last one are not read into anything, whatever they hold,
+ * their outputs and gradients are zero, and the state is the one behind the row's last frame.  No operator keeps anything between
+ * calls, uses atomics or clears memory with a memset: results are the same bits on every run and every call can be captured.  `ws` is
+ * scratch of the caller's, of the size that the operator's _ws_bytes function gives for the same sizes (0: may be NULL). */
+#define AAS_DT_F32 0
+#define AAS_DT_BF16 1
+#define AAS_DT_F16 2
+
+/* Depthwise causal convolution over K = 2, 3 or 4 frames: p[t,n,c] = bias[c] + sum_k weight[c,k] x[t-K+1+k,n,c], y = p or
+ * p sigmoid(p) (silu != 0).  weight [C,K], bias [C] (may be NULL).  state [N,K-1,C] (dtype; may be NULL = zeros): the K-1 frames in
+ * front of the first, oldest first; replaced by the last K-1 frames seen. */
+int aas_causal_conv1d_fwd(aasStream_t stream, int dtype, int T, int N, int C, int K, const void* x, int64_t x_st, int64_t x_sn,
+                          const float* weight, const float* bias, int silu, const int* len, void* state, void* y);
+/* Gradients of the call without a state: dx [T,N,C], dweight [C,K], dbias [C] (each may be NULL).  ws: partial sums. */
+size_t aas_causal_conv1d_bwd_ws_bytes(int T, int N, int C, int K);
+int aas_causal_conv1d_bwd(aasStream_t stream, int dtype, int T, int N, int C, int K, const void* x, int64_t x_st, int64_t x_sn,
+                          const float* weight, const float* bias, int silu, const int* len, const void* dy, int64_t dy_st, int64_t dy_sn,
+                          void* dx, float* dweight, float* dbias, void* ws);
+
+/* Selective state space scan, per row n, channel c and state s (1 <= S <= 64):
+ *   d[t] = softplus(dt[t] + dt_bias)  (softplus = 0: dt + dt_bias),   h_s[t] = exp(d[t] A_s) h_s[t-1] + d[t] x[t] B_s[t],
+ *   o[t] = sum_s C_s[t] h_s[t] + D x[t],   y[t] = o[t] z[t] sigmoid(z[t])  (z = NULL: o[t]).
+ * x, dt, z, y [T,N,Ch]; B, C [T,N,G,S] with channel c reading group c / (Ch / G), strides (time, row, group), state stride 1;
+ * A [Ch,S], D, dt_bias [Ch] fp32 (the last two may be NULL); state [N,Ch,S] fp32 in and out (may be NULL = zeros, dropped). */
+typedef struct aasScan {
+    int size;               /* sizeof(aasScan): checked */
+    int dtype, T, N, Ch, S, G, softplus;
+    const void *x, *dt, *z, *B, *C;
+    const float *A, *D, *dt_bias;
+    const int* len;
+    int64_t x_st, x_sn, dt_st, dt_sn, z_st, z_sn, B_st, B_sn, B_sg, C_st, C_sn, C_sg;
+} aasScan;
+/* hsave (NULL unless a backward pass follows): fp32 [ceil(T/16)][N][Ch][S], receives the state in front of every 16th frame. */
+size_t aas_ssm_scan_fwd_ws_bytes(int T, int N, int Ch, int S, int G);
+int aas_ssm_scan_fwd(aasStream_t stream, const aasScan* d, float* state, void* y, float* hsave, void* ws);
+/* Gradients of the call without a state; hsave as the forward pass left it.  dx, ddt, dz [T,N,Ch]; dB, dC [T,N,G,S]; dA [Ch,S];
+ * dD, ddt_bias [Ch] (dz, dD, ddt_bias may be NULL). */
+size_t aas_ssm_scan_bwd_ws_bytes(int T, int N, int Ch, int S, int G);
+int aas_ssm_scan_bwd(aasStream_t stream, const aasScan* d, const void* dy, int64_t dy_st, int64_t dy_sn, const float* hsave, void* dx, void* ddt,
+                     void* dz, void* dB, void* dC, float* dA, float* dD, float* ddt_bias, void* ws);
+
+/* Residual sum and the norm in front of the next block, one pass (C <= 16384):
+ *   r = residual + scale * drop(x)  (kept in r_dtype: dtype or AAS_DT_F32),   y = (r - mean) rstd weight + bias,
+ * with mean over the row (layer = 1) or 0 (layer = 0), rstd = 1 / sqrt(mean((r - mean)^2) + eps); the norm reads r as it is kept.
+ * residual, weight, bias, scale may be NULL (zeros, ones, zeros, ones; without residual, scale and dropout r may be NULL: it is x).
+ * Dropout: element i of x in row-major order is kept iff its 16 random bits are >= thr (0 <= thr <= 65536; 0 = no dropout), a kept one
+ * is multiplied by 65536 / (65536 - thr).  The bits: counter offset + i / 8 of Philox-4x32-10 (Salmon et al. 2011) under the key `seed`,
+ * word (i % 8) / 2, low half for even i.  d_seed (device int64 [2], may be NULL): {seed, offset} read when the launch runs, in place of
+ * the arguments; seed_used (device int64 [2], may be NULL) receives what was used.
+ * stat [R][2] fp32 receives (mean, rstd); may be NULL. */
+int aas_residual_norm_fwd(aasStream_t stream, int dtype, int r_dtype, int64_t R, int C, const void* x, int64_t x_ld, const void* residual,
+                          int64_t res_ld, const float* weight, const float* bias, const float* scale, float eps, int layer, int thr,
+                          int64_t seed, int64_t offset, const int64_t* d_seed, int64_t* seed_used, void* y, void* r, float* stat);
+/* From dy (gradient of y, may be NULL = zeros) and dr_out (gradient of r, may be NULL): dx [R,C], dresidual [R,C] (r_dtype; may be NULL),
+ * dweight, dbias, dscale [C] (may be NULL).  r as the forward pass kept it; x is read only for dscale. */
+size_t aas_residual_norm_bwd_ws_bytes(int64_t R, int C);
+int aas_residual_norm_bwd(aasStream_t stream, int dtype, int r_dtype, int64_t R, int C, const void* dy, int64_t dy_ld, const void* dr_out,
+                          int64_t dr_ld, const void* r, int64_t r_ld, const void* x, int64_t x_ld, const float* stat, const float* weight,
+                          const float* scale, int layer, int thr, int64_t seed, int64_t offset, const int64_t* d_seed, void* dx,
+                          void* dresidual, float* dweight, float* dbias, float* dscale, void* ws);
+
+/* Root-mean-square norm behind a block with its gate, per group of C / groups channels (<= 16384 channels a group):
+ *   norm_first = 0: y = norm(x silu(gate)) weight;   norm_first = 1: y = norm(x) weight silu(gate),   norm(v) = v / sqrt(mean(v^2) + eps).
+ * x, gate: R rows of pitch x_ld, gate_ld; weight [C] may be NULL (ones). */
+int aas_gated_norm_fwd(aasStream_t stream, int dtype, int64_t R, int C, int groups, const void* x, int64_t x_ld, const void* gate,
+                       int64_t gate_ld, const float* weight, float eps, int norm_first, void* y);
+size_t aas_gated_norm_bwd_ws_bytes(int64_t R, int C, int groups);
+int aas_gated_norm_bwd(aasStream_t stream, int dtype, int64_t R, int C, int groups, const void* dy, int64_t dy_ld, const void* x, int64_t x_ld,
+                       const void* gate, int64_t gate_ld, const float* weight, float eps, int norm_first, void* dx, void* dgate,
+                       float* dweight, void* ws);
+
+/* y = dropout(x) over n elements, the bits as above; the backward pass is the same call on dy with the same seed and offset. */
+int aas_dropout(aasStream_t stream, int dtype, int64_t n, const void* x, void* y, int thr, int64_t seed, int64_t offset,
+                const int64_t* d_seed, int64_t* seed_used);
+
 #ifdef __cplusplus
 }
 #endif
