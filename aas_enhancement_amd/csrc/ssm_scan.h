@@ -26,6 +26,19 @@ struct ScanDev {                 // aasScan with the pointers' types left to the
     int64_t x_st, x_sn, dt_st, dt_sn, z_st, z_sn, B_st, B_sn, B_sg, C_st, C_sn, C_sg;
 };
 
+// Splitting the time axis.  With few rows and channels a launch of one workgroup per (row, 64 channels) leaves most of the chip idle while
+// each walks the whole sequence.  The axis is then cut into chunks of whole tiles: a first launch (scan_carry.h) forms what each chunk
+// adds to the state - its own end, from zero - and the sum of its d; the state in front of chunk k is the ends of the chunks before it,
+// each decayed by exp(A sum of d) of the chunks between, which every workgroup of the main launch folds for itself.  The decays are
+// formed once more than unsplit, so it pays only where the chip is far from full.
+struct ScanChunks { int n, tiles; };
+ScanChunks scan_chunks(int T, int N, int Ch, int G, int want_blocks);
+
+// h in front of chunk k (REV: the carry behind it) from the chunks' ends [nchunk][N][Ch][S] and sums of d [nchunk][N][Ch]
+template <int NG, bool REV>
+__device__ __forceinline__ void scan_fold(f32x4 (&h)[NG], const f32x4 (&A2)[NG], const float* ends, const float* sums, int k, int nchunk, int64_t rows,
+                                          int64_t ch, int S, int q, bool svec);
+
 struct ScanBlock {               // where a workgroup stands
     int n, grp, c0, cn;          // row, group of B / C, first channel, channels (<= 64)
 };
@@ -89,6 +102,25 @@ __device__ __forceinline__ void scan_put_states4(float* row, int s0, int S, bool
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (s0 + j < S) row[s0 + j] = v[j];
+}
+
+template <int NG, bool REV>
+__device__ __forceinline__ void scan_fold(f32x4 (&h)[NG], const f32x4 (&A2)[NG], const float* ends, const float* sums, int k, int nchunk, int64_t rows,
+                                          int64_t ch, int S, int q, bool svec) {
+    // forward: chunk j's own end for j = 0 .. k-1, the newest last;  REV: j = nchunk-1 .. k+1
+    const int first = REV ? nchunk - 1 : 0, count = REV ? nchunk - 1 - k : k;
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) {
+        const int j = REV ? first - i : first + i;
+        const int64_t at = j * rows + ch;
+        const float d = sums[at];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const f32x4 e = scan_states4(ends + at * S, g * 16 + 4 * q, S, svec);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) h[g][m] = i == 0 ? e[m] : fmaf(__builtin_amdgcn_exp2f(d * A2[g][m]), h[g][m], e[m]);
+        }
+    }
 }
 
 // host side

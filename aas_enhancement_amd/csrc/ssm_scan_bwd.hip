@@ -9,7 +9,7 @@
 // states x {dB, dC}) over the 16 channels of a wave go by exchanges that halve the number of values with the number of lanes still to
 // add (lane halves, rows of 16, then within the row), then over the four waves through LDS, then - plain stores, no atomics - over the
 // workgroups by a second launch.
-#include "ssm_scan.h"
+#include "scan_carry.h"
 
 namespace {
 
@@ -39,7 +39,8 @@ __device__ __forceinline__ float sum_channels8(const float v[8], bool bit3) {
 template <class T, int NG, bool VEC>
 __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __restrict__ dy, int64_t dy_st, int64_t dy_sn, const float* __restrict__ hsave,
                                                        T* __restrict__ dx, T* __restrict__ ddt, T* __restrict__ dz, float* __restrict__ part_bc,
-                                                       float* __restrict__ part_a, float* __restrict__ part_d) {
+                                                       float* __restrict__ part_a, float* __restrict__ part_d,
+                                                       const float* __restrict__ ends, const float* __restrict__ sums) {
     __shared__ float2 dd[SCAN_TT][SCAN_CH];             // d, d x
     __shared__ float go[SCAN_TT][SCAN_CH];
     __shared__ __align__(16) float bs[SCAN_TT][NG * 16], cs[SCAN_TT][NG * 16];
@@ -65,6 +66,9 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
         A2[g] = on ? scan_states4(a.A + (int64_t)(b.c0 + cw) * a.S, g * 16 + 4 * q, a.S, svec) * SCAN_LOG2E : zero;
         dA[g] = carry[g] = zero;
     }
+    const int chunk = blockIdx.y;
+    if (on && chunk + 1 < a.nchunk)
+        scan_fold<NG, true>(carry, A2, ends, sums, chunk, a.nchunk, (int64_t)a.N * a.Ch, (int64_t)b.n * a.Ch + b.c0 + cw, a.S, q, svec);
     const f32x4 bias = a.dt_bias ? load4n<float, false>(a.dt_bias + b.c0 + lc, ln) : zero;
     const f32x4 Dv = a.D ? load4n<float, false>(a.D + b.c0 + lc, ln) : zero;
     f32x4 dD = zero, dbias = zero;
@@ -87,12 +91,13 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
             h0[g] = on ? scan_states4(hsave + ((int64_t)tile * a.N * a.Ch) * a.S + srow, g * 16 + 4 * q, a.S, svec) : zero;
         }
     };
-    const int tiles = (L + SCAN_TT - 1) / SCAN_TT;
+    const int all = (L + SCAN_TT - 1) / SCAN_TT, k0 = chunk * a.tiles_per_chunk;
+    const int k1 = k0 + a.tiles_per_chunk, tiles = k1 < all ? k1 : all;                       // tiles [k0, tiles) have frames, up to k1 are written
     const int64_t orow = (int64_t)a.N * a.Ch, obase = (int64_t)b.n * a.Ch + b.c0 + lc;
     const int nblk = a.nbg;
     const int cb = (b.c0 - b.grp * a.cpg) / SCAN_CH;
-    if (tiles > 0) load(tiles - 1);
-    for (int k = tiles - 1; k >= 0; --k) {
+    if (tiles > k0) load(tiles - 1);
+    for (int k = tiles - 1; k >= k0; --k) {
         const int64_t t = (int64_t)k * SCAN_TT + lr;
         const bool live = t < L;
         const f32x4 xe = xr, te = tr, ze = zr, ge = gr;
@@ -111,7 +116,7 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
             cs[lr][g * 16 + (tid & 15)] = cr[g];
             h[g] = h0[g];
         }
-        if (k > 0) load(k - 1);
+        if (k > k0) load(k - 1);
         __syncthreads();
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -212,7 +217,8 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
                     (bc[0][f][j] + bc[1][f][j]) + (bc[2][f][j] + bc[3][f][j]);
         }
     }
-    for (int64_t t = (int64_t)tiles * SCAN_TT + lr; t < a.T; t += SCAN_TT) {
+    const int te = chunk + 1 == a.nchunk || (int64_t)k1 * SCAN_TT > a.T ? a.T : k1 * SCAN_TT;
+    for (int64_t t = (int64_t)(tiles > k0 ? tiles : k0) * SCAN_TT + lr; t < te; t += SCAN_TT) {
         const int64_t at = t * orow + obase;
         store4n<T, VEC>(dx + at, zero, ln);
         store4n<T, VEC>(ddt + at, zero, ln);
@@ -220,7 +226,7 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
     }
     if (on)
 #pragma unroll
-        for (int g = 0; g < NG; ++g) scan_put_states4(part_a + srow, g * 16 + 4 * q, a.S, svec, dA[g]);
+        for (int g = 0; g < NG; ++g) scan_put_states4(part_a + (int64_t)chunk * a.N * a.Ch * a.S + srow, g * 16 + 4 * q, a.S, svec, dA[g]);
     __syncthreads();                                                    // (the last tile's readers of us, ws)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -234,7 +240,7 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
         float v = 0.f;
 #pragma unroll
         for (int i = 0; i < SCAN_TT; ++i) v += from[i][c];
-        if (c < b.cn) part_d[((int64_t)b.n * 2 + (tid >= SCAN_CH ? 1 : 0)) * a.Ch + b.c0 + c] = v;
+        if (c < b.cn) part_d[(((int64_t)chunk * a.N + b.n) * 2 + (tid >= SCAN_CH ? 1 : 0)) * a.Ch + b.c0 + c] = v;
     }
 }
 
@@ -258,29 +264,35 @@ __global__ __launch_bounds__(256) void scan_bc_kernel(const float* __restrict__ 
     }
 }
 
-struct BwdWs { size_t bc, a, d, total; };               // byte offsets
+ScanChunks bwd_chunks(int T, int N, int Ch, int G) { return scan_chunks(T, N, Ch, G, 512); }
+
+struct BwdWs { size_t bc, a, d, ends, sums, total; };   // byte offsets
 BwdWs bwd_ws(int T, int N, int Ch, int S, int G) {
     BwdWs w;
+    const int n = bwd_chunks(T, N, Ch, G).n;
     auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     w.bc = 0;
     w.a = up((size_t)T * N * G * cdiv(Ch / G, SCAN_CH) * 2 * S * sizeof(float));
-    w.d = w.a + up((size_t)N * Ch * S * sizeof(float));
-    w.total = w.d + up((size_t)N * 2 * Ch * sizeof(float));
+    w.d = w.a + up((size_t)n * N * Ch * S * sizeof(float));
+    w.ends = w.d + up((size_t)n * N * 2 * Ch * sizeof(float));
+    w.sums = w.ends + (n > 1 ? up((size_t)n * N * Ch * S * sizeof(float)) : 0);
+    w.total = w.sums + (n > 1 ? up((size_t)n * N * Ch * sizeof(float)) : 0);
     return w;
 }
 
 template <class T>
 void launch_bwd(hipStream_t s, const ScanDev& a, bool vec, const void* dy, int64_t dy_st, int64_t dy_sn, const float* hsave, void* dx, void* ddt, void* dz,
-                float* bc, float* pa, float* pd) {
-    const dim3 grid((unsigned)((int64_t)a.N * a.nbg * a.G));
+                float* bc, float* pa, float* pd, float* ends, float* sums) {
+    if (a.nchunk > 1) launch_carry<T, true>(s, a, vec, nullptr, dy, dy_st, dy_sn, ends, sums);
+    const dim3 grid((unsigned)((int64_t)a.N * a.nbg * a.G), a.nchunk);
 #define AAS_GO(NG_)                                                                                                                   \
     do {                                                                                                                              \
         if (vec)                                                                                                                      \
             hipLaunchKernelGGL((scan_bwd_kernel<T, NG_, true>), grid, dim3(256), 0, s, a, (const T*)dy, dy_st, dy_sn, hsave, (T*)dx,  \
-                               (T*)ddt, (T*)dz, bc, pa, pd);                                                                          \
+                               (T*)ddt, (T*)dz, bc, pa, pd, ends, sums);                                                                          \
         else                                                                                                                          \
             hipLaunchKernelGGL((scan_bwd_kernel<T, NG_, false>), grid, dim3(256), 0, s, a, (const T*)dy, dy_st, dy_sn, hsave, (T*)dx, \
-                               (T*)ddt, (T*)dz, bc, pa, pd);                                                                          \
+                               (T*)ddt, (T*)dz, bc, pa, pd, ends, sums);                                                                          \
     } while (0)
     if (a.S <= 16) AAS_GO(1);
     else if (a.S <= 32) AAS_GO(2);
@@ -303,18 +315,22 @@ extern "C" int aas_ssm_scan_bwd(aasStream_t stream, const aasScan* d, const void
     const bool empty = d->T == 0 || d->N == 0;
     if (d->Ch == 0) return 0;
     AAS_CHECK(dA != nullptr, "%s: null pointer", who);
-    const BwdWs w = empty ? BwdWs{0, 0, 0, 0} : bwd_ws(d->T, d->N, d->Ch, d->S, d->G);
+    const BwdWs w = empty ? BwdWs{0, 0, 0, 0, 0, 0} : bwd_ws(d->T, d->N, d->Ch, d->S, d->G);
+    const ScanChunks ck = empty ? ScanChunks{0, 0} : bwd_chunks(d->T, d->N, d->Ch, d->G);
     char* base = (char*)ws;
     if (!empty) {
         AAS_CHECK(dy && hsave && dx && ddt && dB && dC && ws && (dz || !d->z), "%s: null pointer", who);
         AAS_CHECK(aas_aligned(hsave, 16) && aas_aligned(ws, 16), "%s: hsave and ws must be 16-byte aligned", who);
         ScanDev a;
         scan_dev(d, &a);
+        a.nchunk = ck.n;
+        a.tiles_per_chunk = ck.tiles;
         const int al = 4 * aas_dt_size(d->dtype);
         const bool vec = scan_vec(a, d->dtype) && dy_st % 4 == 0 && dy_sn % 4 == 0 && aas_aligned(dy, al) && aas_aligned(dx, al) && aas_aligned(ddt, al) &&
                          (!dz || aas_aligned(dz, al));
         AAS_DT_SWITCH(d->dtype, E, launch_bwd<E>(s, a, vec, dy, dy_st, dy_sn, hsave, dx, ddt, d->z ? dz : nullptr, (float*)(base + w.bc),
-                                                 (float*)(base + w.a), (float*)(base + w.d)));
+                                                 (float*)(base + w.a), (float*)(base + w.d), (float*)(base + w.ends),
+                                                 (float*)(base + w.sums)));
         AAS_LAUNCH_CHECK(who);
         const int64_t total = (int64_t)d->T * d->N * d->G * d->S;
         const int blocks = (int)(total / 256 + 1 < 4096 ? total / 256 + 1 : 4096);
@@ -322,7 +338,7 @@ extern "C" int aas_ssm_scan_bwd(aasStream_t stream, const aasScan* d, const void
                                                       d->S, a.nbg, d->len, (E*)dB, (E*)dC));
         AAS_LAUNCH_CHECK(who);
     }
-    const int P = empty ? 0 : d->N;
+    const int P = empty ? 0 : d->N * ck.n;
     ColMap ma = {{dA, nullptr, nullptr, nullptr}, {d->Ch * d->S, 0, 0, 0}, 0, 1};
     if (aas_sum_partials(s, (const float*)(base + w.a), P, d->Ch * d->S, ma, who)) return 2;
     if (!dD && !ddt_bias) return 0;

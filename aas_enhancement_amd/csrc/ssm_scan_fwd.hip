@@ -1,10 +1,11 @@
 // Selective state space scan, forward (ssm_scan.h has the mathematics and the layout).
-#include "ssm_scan.h"
+#include "scan_carry.h"
 
 namespace {
 
 template <class T, int NG, bool VEC>
-__global__ __launch_bounds__(256) void scan_fwd_kernel(ScanDev a, float* __restrict__ state, T* __restrict__ y, float* __restrict__ hsave) {
+__global__ __launch_bounds__(256) void scan_fwd_kernel(ScanDev a, float* __restrict__ state, T* __restrict__ y, float* __restrict__ hsave,
+                                                       const float* __restrict__ ends, const float* __restrict__ sums) {
     __shared__ float2 dd[2][SCAN_TT][SCAN_CH];          // d, d x
     __shared__ __align__(16) float bs[2][SCAN_TT][NG * 16], cs[2][SCAN_TT][NG * 16];
     __shared__ float ys[2][SCAN_TT][SCAN_YP];
@@ -27,9 +28,14 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanDev a, float* __restr
         A2[g] = h[g] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (on) {
             A2[g] = scan_states4(a.A + (int64_t)(b.c0 + cw) * a.S, s0, a.S, svec) * SCAN_LOG2E;
-            if (state) h[g] = scan_states4(state + srow, s0, a.S, svec);
+            // (a split launch: the first chunk's end has the state in it; and the last chunk, which writes the new state, may finish first, so
+            // the first one reads the copy that the carry launch left)
+            if (state && a.nchunk == 1) h[g] = scan_states4(state + srow, s0, a.S, svec);
+            if (state && a.nchunk > 1 && blockIdx.y == 0) h[g] = scan_states4(ends + ((int64_t)(a.nchunk - 1) * a.N * a.Ch) * a.S + srow, s0, a.S, svec);
         }
     }
+    if (on && blockIdx.y > 0)
+        scan_fold<NG, false>(h, A2, ends, sums, blockIdx.y, a.nchunk, (int64_t)a.N * a.Ch, (int64_t)b.n * a.Ch + b.c0 + cw, a.S, q, svec);
     const f32x4 bias = a.dt_bias ? load4n<float, false>(a.dt_bias + b.c0 + lc, ln) : f32x4{0.f, 0.f, 0.f, 0.f};
     const f32x4 Dv = a.D ? load4n<float, false>(a.D + b.c0 + lc, ln) : f32x4{0.f, 0.f, 0.f, 0.f};
 
@@ -62,18 +68,19 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanDev a, float* __restr
             cs[u][lr][g * 16 + (tid & 15)] = cr[g];
         }
     };
-    const int tiles = (L + SCAN_TT - 1) / SCAN_TT;
-    T* yp = y + ((int64_t)lr * a.N + b.n) * a.Ch + b.c0 + lc;
+    const int all = (L + SCAN_TT - 1) / SCAN_TT, k0 = blockIdx.y * a.tiles_per_chunk;
+    const int k1 = k0 + a.tiles_per_chunk, tiles = k1 < all ? k1 : all;                       // tiles [k0, tiles) have frames, up to k1 are written
+    T* yp = y + ((int64_t)(k0 * SCAN_TT + lr) * a.N + b.n) * a.Ch + b.c0 + lc;
     const int64_t ytile = (int64_t)SCAN_TT * a.N * a.Ch;
-    if (tiles > 0) {
-        load(0);
-        stage(0, 0);
+    if (tiles > k0) {
+        load(k0);
+        stage(k0, k0 & 1);
         xe = xr;
         ze = zr;
-        if (tiles > 1) load(1);
+        if (tiles > k0 + 1) load(k0 + 1);
         __syncthreads();
     }
-    for (int k = 0; k < tiles; ++k, yp += ytile) {
+    for (int k = k0; k < tiles; ++k, yp += ytile) {
         const int u = k & 1;
         if (hsave && on) {
             float* hp = hsave + ((int64_t)k * a.N * a.Ch) * a.S + srow;
@@ -122,19 +129,21 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanDev a, float* __restr
         xe = xn;
         ze = zn;
     }
-    for (int t = tiles * SCAN_TT + lr; t < a.T; t += SCAN_TT, yp += ytile) store4n<T, VEC>(yp, f32x4{0.f, 0.f, 0.f, 0.f}, ln);
-    if (state && on)
+    const int te = blockIdx.y + 1 == gridDim.y || (int64_t)k1 * SCAN_TT > a.T ? a.T : k1 * SCAN_TT;
+    for (int t = (tiles > k0 ? tiles : k0) * SCAN_TT + lr; t < te; t += SCAN_TT, yp += ytile) store4n<T, VEC>(yp, f32x4{0.f, 0.f, 0.f, 0.f}, ln);
+    if (state && on && blockIdx.y + 1 == gridDim.y)
 #pragma unroll
         for (int g = 0; g < NG; ++g) scan_put_states4(state + srow, g * 16 + 4 * q, a.S, svec, h[g]);
 }
 
 template <class T>
-void launch_fwd(hipStream_t s, const ScanDev& a, bool vec, float* state, void* y, float* hsave) {
-    const dim3 grid((unsigned)((int64_t)a.N * a.nbg * a.G));
+void launch_fwd(hipStream_t s, const ScanDev& a, bool vec, float* state, void* y, float* hsave, float* ends, float* sums) {
+    if (a.nchunk > 1) launch_carry<T, false>(s, a, vec, state, nullptr, 0, 0, ends, sums);
+    const dim3 grid((unsigned)((int64_t)a.N * a.nbg * a.G), a.nchunk);
 #define AAS_GO(NG_)                                                                                                                   \
     do {                                                                                                                              \
-        if (vec) hipLaunchKernelGGL((scan_fwd_kernel<T, NG_, true>), grid, dim3(256), 0, s, a, state, (T*)y, hsave);                  \
-        else hipLaunchKernelGGL((scan_fwd_kernel<T, NG_, false>), grid, dim3(256), 0, s, a, state, (T*)y, hsave);                     \
+        if (vec) hipLaunchKernelGGL((scan_fwd_kernel<T, NG_, true>), grid, dim3(256), 0, s, a, state, (T*)y, hsave, ends, sums);                  \
+        else hipLaunchKernelGGL((scan_fwd_kernel<T, NG_, false>), grid, dim3(256), 0, s, a, state, (T*)y, hsave, ends, sums);                     \
     } while (0)
     if (a.S <= 16) AAS_GO(1);
     else if (a.S <= 32) AAS_GO(2);
@@ -163,7 +172,7 @@ void scan_dev(const aasScan* d, ScanDev* a) {
     a->cpg = d->Ch / d->G;
     a->nbg = cdiv(a->cpg, SCAN_CH);
     a->tiles_per_chunk = scan_tiles(d->T);
-    a->nchunk = 1;
+    a->nchunk = 1;                                      // (set by the launcher)
     a->svec = d->S % 4 == 0 && aas_aligned(d->A, 16);
     a->x = d->x; a->dt = d->dt; a->z = d->z; a->B = d->B; a->C = d->C;
     a->A = d->A; a->D = d->D; a->dt_bias = d->dt_bias; a->len = d->len;
@@ -179,18 +188,44 @@ bool scan_vec(const ScanDev& a, int dtype) {
            aas_aligned(a.dt, al) && (!a.z || (a.z_st % 4 == 0 && a.z_sn % 4 == 0 && aas_aligned(a.z, al)));
 }
 
-extern "C" size_t aas_ssm_scan_fwd_ws_bytes(int T, int N, int Ch, int S, int G) { return 0; }
+ScanChunks scan_chunks(int T, int N, int Ch, int G, int want_blocks) {
+    const int tiles = scan_tiles(T);
+    const int64_t blocks = (int64_t)N * cdiv(Ch / G, SCAN_CH) * G;
+    ScanChunks c = {1, tiles};
+    if (blocks == 0 || blocks * 2 > want_blocks) return c;
+    int n = (int)(want_blocks / blocks);
+    if (n > 32) n = 32;
+    if (n > tiles / 4) n = tiles / 4;                   // at least four tiles a chunk
+    if (n < 3) return c;                                // (two chunks: the carry launch and half of the main one take as long as the whole)
+    c.tiles = cdiv(tiles, n);
+    c.n = cdiv(tiles, c.tiles);
+    return c;
+}
+
+static ScanChunks fwd_chunks(int T, int N, int Ch, int G) { return scan_chunks(T, N, Ch, G, 1024); }
+
+extern "C" size_t aas_ssm_scan_fwd_ws_bytes(int T, int N, int Ch, int S, int G) {
+    if (T <= 0 || N <= 0 || Ch <= 0 || S <= 0 || G <= 0 || Ch % G) return 0;
+    const int n = fwd_chunks(T, N, Ch, G).n;
+    return n == 1 ? 0 : (size_t)n * N * Ch * (S + 1) * sizeof(float);
+}
 
 extern "C" int aas_ssm_scan_fwd(aasStream_t stream, const aasScan* d, float* state, void* y, float* hsave, void* ws) {
     if (scan_check("aas_ssm_scan_fwd", d)) return 1;
     if (d->T == 0 || d->N == 0 || d->Ch == 0) return 0;
     AAS_CHECK(y != nullptr, "aas_ssm_scan_fwd: null pointer");
-    AAS_CHECK(aas_aligned(hsave, 16), "aas_ssm_scan_fwd: hsave must be 16-byte aligned");
+    AAS_CHECK(aas_aligned(hsave, 16) && aas_aligned(ws, 16), "aas_ssm_scan_fwd: hsave and ws must be 16-byte aligned");
     ScanDev a;
     scan_dev(d, &a);
+    const ScanChunks c = fwd_chunks(d->T, d->N, d->Ch, d->G);
+    AAS_CHECK(c.n == 1 || ws, "aas_ssm_scan_fwd: ws is wanted");
+    a.nchunk = c.n;
+    a.tiles_per_chunk = c.tiles;
     if (!aas_aligned(state, 16)) a.svec = 0;
     const bool vec = scan_vec(a, d->dtype) && aas_aligned(y, 4 * aas_dt_size(d->dtype));
-    AAS_DT_SWITCH(d->dtype, E, launch_fwd<E>((hipStream_t)stream, a, vec, state, y, hsave));
+    float* ends = (float*)ws;
+    float* sums = ends ? ends + (int64_t)c.n * d->N * d->Ch * d->S : nullptr;
+    AAS_DT_SWITCH(d->dtype, E, launch_fwd<E>((hipStream_t)stream, a, vec, state, y, hsave, ends, sums));
     AAS_LAUNCH_CHECK("aas_ssm_scan_fwd");
     return 0;
 }

@@ -137,7 +137,7 @@ def test_conv_stream_equals_whole(ops):
 
 # -------------------------------------------------------------------------------------------------------------------------- scan
 SCAN = [(1, 1, 1, 1, 1), (1, 3, 70, 16, 1), (2, 2, 8, 5, 1), (15, 3, 5, 16, 1), (16, 1, 64, 16, 1), (17, 4, 66, 8, 2), (33, 3, 130, 16, 1),
-        (50, 2, 24, 32, 3), (20, 2, 68, 64, 1), (200, 3, 20, 16, 1)]
+        (50, 2, 24, 32, 3), (20, 2, 68, 64, 1), (200, 3, 20, 16, 1), (333, 4, 70, 5, 1), (700, 1, 12, 64, 2), (530, 2, 65, 24, 1)]
 
 
 def scan_inputs(T, N, Ch, S, G, dtype, lengths=True):
