@@ -161,40 +161,8 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(int TT, int N, int C, int
     }
 }
 
-// 16 columns x 16 row lanes
 __global__ __launch_bounds__(256) void sum_partials_kernel(const float* __restrict__ part, int P, int M, ColMap map) {
-    __shared__ float s[16][17];
-    const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4;
-    const int m = blockIdx.x * 16 + cl;
-    float v = 0.f;
-    if (m < M) {
-        const float* p = part + m;
-        int r = rl;
-        for (; r + 7 * 16 < P; r += 8 * 16) {         // eight loads in flight
-            float u[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) u[i] = p[(int64_t)(r + 16 * i) * M];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v += u[i];
-        }
-        for (; r < P; r += 16) v += p[(int64_t)r * M];
-    }
-    s[rl][cl] = v;
-    __syncthreads();
-    if (rl == 0 && m < M) {
-        float t = s[0][cl];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) t += s[i][cl];
-        int col = m, seg = 0;
-        while (seg + 1 < map.n && col >= map.cols[seg]) { col -= map.cols[seg]; ++seg; }
-        if (map.out[seg]) {
-            if (seg == 0 && map.inner > 0) {
-                const int w = map.cols[0] / map.inner;     // partial row [inner][w] -> out [w][inner]
-                col = (col % w) * map.inner + col / w;
-            }
-            map.out[seg][col] = t;
-        }
-    }
+    sum_columns(part, P, M, map, blockIdx.x);
 }
 
 // Stretch of the time axis per thread: long enough that the K - 1 overlapping frames cost little, short enough that the launch has the

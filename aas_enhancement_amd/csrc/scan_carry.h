@@ -10,18 +10,18 @@ namespace {
 template <class T, int NG, bool VEC, bool REV>
 __global__ __launch_bounds__(256) void scan_carry_kernel(ScanDev a, const float* __restrict__ state, const T* __restrict__ dy, int64_t dy_st, int64_t dy_sn,
                                                          float* __restrict__ ends, float* __restrict__ sums) {
-    __shared__ float2 dd[2][SCAN_TT][SCAN_CH];          // d, and d x (REV: go)
+    __shared__ __align__(16) float2 dd[2][SCAN_TT][SCAN_CH];          // d, and d x (REV: go)
     __shared__ __align__(16) float bs[2][SCAN_TT][NG * 16];
     const ScanBlock b = scan_block(a);
     const int k = blockIdx.y + (REV ? 1 : 0);
     const int tid = threadIdx.x, q = tid & 3, cw = tid >> 2;
-    const int lr = tid >> 4, lc = (tid & 15) * 4, ln = b.cn - lc;
+    const int lr = tid >> 4, lc = (tid & 15) * 4, ln = b.cn - lc, ls = tid & 15;
     const int L = row_length(a.len, b.n, a.T);
     const bool on = cw < b.cn, svec = a.svec != 0;
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    const T* tp = (const T*)a.dt + b.n * a.dt_sn + b.c0 + lc;
-    const T* vp = REV ? dy + b.n * dy_sn + b.c0 + lc : (const T*)a.x + b.n * a.x_sn + b.c0 + lc;
-    const T* zp = REV && a.z ? (const T*)a.z + b.n * a.z_sn + b.c0 + lc : nullptr;
+    const T* tp = (const T*)a.dt + b.n * a.dt_sn + b.c0;
+    const T* vp = REV ? dy + b.n * dy_sn + b.c0 : (const T*)a.x + b.n * a.x_sn + b.c0;
+    const T* zp = REV && a.z ? (const T*)a.z + b.n * a.z_sn + b.c0 : nullptr;
     const T* bp = REV ? (const T*)a.C + b.n * a.C_sn + b.grp * a.C_sg : (const T*)a.B + b.n * a.B_sn + b.grp * a.B_sg;
     const int64_t v_st = REV ? dy_st : a.x_st, b_st = REV ? a.C_st : a.B_st;
     const int64_t rows = (int64_t)a.N * a.Ch, ch = (int64_t)b.n * a.Ch + b.c0 + cw;
@@ -39,29 +39,27 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(ScanDev a, const float*
     const int tiles = (L + SCAN_TT - 1) / SCAN_TT, t0 = k * a.tiles_per_chunk;
     const int t1 = t0 + a.tiles_per_chunk < tiles ? t0 + a.tiles_per_chunk : tiles;
     auto tile_of = [&](int i) { return REV ? t1 - 1 - i : t0 + i; };
-    auto load = [&](int tile) {
-        const int64_t t = (int64_t)tile * SCAN_TT + lr;
-        const int m = t < L ? ln : 0;
-        tr = load4n<T, VEC>(tp + t * a.dt_st, m);
-        vr = load4n<T, VEC>(vp + t * v_st, m);
-        if (zp) zr = load4n<T, VEC>(zp + t * a.z_st, m);
+    const ScanCols<VEC> cols(lc, b.cn);
+    auto load = [&](int tile) {                         // (a frame behind the row's end: its last one, dropped again in stage)
+        const int f = tile * SCAN_TT + lr;
+        const int64_t t = f < L ? f : L - 1;
+        tr = cols.get(tp + t * a.dt_st);
+        vr = cols.get(vp + t * v_st);
+        if (zp) zr = cols.get(zp + t * a.z_st);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const int s = g * 16 + (tid & 15);
-            br[g] = t < L && s < a.S ? (float)bp[t * b_st + s] : 0.f;
-        }
+        for (int g = 0; g < NG; ++g) br[g] = (float)bp[t * b_st + (g * 16 + ls < a.S ? g * 16 + ls : 0)];
     };
     auto stage = [&](int tile, int u) {
-        const bool live = tile * SCAN_TT + lr < L;
+        const bool live = tile * SCAN_TT + lr < L;      // behind the end: d = 0 leaves the state as it is
+        const f32x4 d = cols.keep(scan_delta4(tr, bias, a.softplus), live);
+        f32x4 v = cols.keep(vr, live);
+        sum += d;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float d = live && i < ln ? scan_delta(tr[i], bias[i], a.softplus) : 0.f;
-            sum[i] += d;
-            const float v = REV ? (zp ? vr[i] * (zr[i] * sigm(zr[i])) : vr[i]) : d * vr[i];
-            dd[u][lr][lc + i] = make_float2(d, v);
-        }
+        for (int i = 0; i < 4; ++i) v[i] *= REV ? (zp ? zr[i] * sigm(zr[i]) : 1.f) : d[i];
+        if (REV) v = cols.keep(v, live);
+        scan_stage(&dd[u][lr][lc], d, v);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) bs[u][lr][g * 16 + (tid & 15)] = br[g];
+        for (int g = 0; g < NG; ++g) bs[u][lr][g * 16 + ls] = live && g * 16 + ls < a.S ? br[g] : 0.f;
     };
     const int n = t1 - t0;
     if (n > 0) {

@@ -54,14 +54,48 @@ __device__ __forceinline__ int row_length(const int* len, int n, int T) {   // a
     return v < 0 ? 0 : (v > T ? T : v);
 }
 
-// out[map(m)] = sum over p of part[p][m], p in order within 16 interleaved chains and the chains joined in order: the same bits on
-// every run.  16 columns x 16 row lanes per workgroup: a few hundred partial rows are a few rounds of loads in flight.
+// Sums over partial rows: out[map(m)] = sum over p of part[p][m], in 16 interleaved chains over p that are joined in order: the same
+// bits on every run.  A workgroup takes 16 columns with 16 row lanes: a few hundred partial rows are a few rounds of loads in flight.
 struct ColMap {                 // column m of a partial row -> where its sum goes: segment i holds cols[i] columns
     float* out[4];
     int cols[4];
-    int inner;                  // > 0: segment 0 is stored [cols / inner][inner] in the partial row and [inner][cols / inner] in out[0]
+    int inner;                  // > 0: segment 0 is stored [inner][cols / inner] in the partial row and [cols / inner][inner] in out[0]
     int n;
 };
+__device__ __forceinline__ void sum_columns(const float* __restrict__ part, int P, int M, const ColMap& map, int block) {
+    __shared__ float s[16][17];
+    const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4;
+    const int m = block * 16 + cl;
+    float v = 0.f;
+    if (m < M) {
+        const float* p = part + m;
+        int r = rl;
+        for (; r + 7 * 16 < P; r += 8 * 16) {         // eight loads in flight
+            float u[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] = p[(int64_t)(r + 16 * i) * M];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v += u[i];
+        }
+        for (; r < P; r += 16) v += p[(int64_t)r * M];
+    }
+    s[rl][cl] = v;
+    __syncthreads();
+    if (rl == 0 && m < M) {
+        float t = s[0][cl];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) t += s[i][cl];
+        int col = m, seg = 0;
+        while (seg + 1 < map.n && col >= map.cols[seg]) { col -= map.cols[seg]; ++seg; }
+        if (map.out[seg]) {
+            if (seg == 0 && map.inner > 0) {
+                const int w = map.cols[0] / map.inner;
+                col = (col % w) * map.inner + col / w;
+            }
+            map.out[seg][col] = t;
+        }
+    }
+}
 int aas_sum_partials(hipStream_t s, const float* part, int P, int M, const ColMap& map, const char* who);
 
 #define AAS_DT_SWITCH(code, T, ...)                                   \

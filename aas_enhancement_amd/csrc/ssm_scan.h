@@ -55,35 +55,74 @@ __device__ __forceinline__ ScanBlock scan_block(const ScanDev& a) {
     return b;
 }
 
-// log(1 + e^-|v|) + max(v, 0), with e = e^-|v| also handed back.  log(1 + e) = 2 atanh(e / (2 + e)) as its series: e <= 1, so the argument
-// is at most 1/3 and nine terms leave 3^-20 / 19 of the sum - full relative accuracy also where e is tiny (d of 1e-3 and below), which
-// log2(1 + e) in fp32 has not.
-__device__ __forceinline__ float softplusf_(float v, float* e_out) {
-    const float e = expf(-fabsf(v));
-    *e_out = e;
+// The four neighbouring channels of the loading thread, brought inside the workgroup's: loads need no branches, what lies outside is
+// replaced by zeros behind them.  Frames are brought inside the row in the same way.
+template <bool VEC> struct ScanCols {
+    int c[VEC ? 1 : 4];
+    bool in[VEC ? 1 : 4];
+    __device__ __forceinline__ ScanCols(int lc, int cn) {
+#pragma unroll
+        for (int i = 0; i < (VEC ? 1 : 4); ++i) {
+            in[i] = lc + i < cn;
+            c[i] = in[i] ? lc + i : (VEC ? cn - 4 : cn - 1);
+        }
+    }
+    template <class T> __device__ __forceinline__ f32x4 get(const T* row) const {
+        if (VEC) return load4(row + c[0]);
+        f32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (float)row[c[VEC ? 0 : i]];
+        return v;
+    }
+    __device__ __forceinline__ f32x4 keep(f32x4 v, bool live) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = live && in[VEC ? 0 : i] ? v[i] : 0.f;
+        return v;
+    }
+};
+
+// d = softplus(v) = max(v, 0) + log(1 + e), e = e^-|v|, and its derivative.  log(1 + e) = 2 atanh(e / (2 + e)): the argument s is at most
+// 1/3 and atanh(s) / s a polynomial in s^2 (Chebyshev interpolation, off by 4e-9), so d keeps full relative accuracy where e is tiny (d
+// of 1e-3 and below), which log(1 + e) formed in fp32 has not.  The exponential takes the rounding of v log2(e) along.
+__device__ __forceinline__ float scan_softplus(float v, float* slope) {
+    const float m = fabsf(v), p = m * SCAN_LOG2E;
+    const float lost = fmaf(m, SCAN_LOG2E, -p) + m * 1.925963033500e-8f;                // m log2(e) - p
+    float e = __builtin_amdgcn_exp2f(-p);
+    e = fmaf(e, -SCAN_LN2 * lost, e);
     const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
-    float p = 1.f / 17.f;
-    p = fmaf(p, q, 1.f / 15.f);
-    p = fmaf(p, q, 1.f / 13.f);
-    p = fmaf(p, q, 1.f / 11.f);
-    p = fmaf(p, q, 1.f / 9.f);
-    p = fmaf(p, q, 1.f / 7.f);
-    p = fmaf(p, q, 1.f / 5.f);
-    p = fmaf(p, q, 1.f / 3.f);
-    p = fmaf(p, q, 1.f);
-    return fmaf(2.f * s, p, fmaxf(v, 0.f));
+    float y = fmaf(0.14078889f, q, 0.13982579f);
+    y = fmaf(y, q, 0.20012298f);
+    y = fmaf(y, q, 0.33333161f);
+    y = fmaf(y, q, 1.f);
+    if (slope) {
+        const float r = __builtin_amdgcn_rcpf(1.f + e);
+        *slope = v >= 0.f ? r : e * r;
+    }
+    return fmaf(2.f * s, y, fmaxf(v, 0.f));             // (a NaN comes through y)
 }
-// d and, for the backward pass, its derivative
-__device__ __forceinline__ float scan_delta(float dt, float bias, int softplus) {
-    const float v = dt + bias;
-    if (!softplus) return v;
-    float e;
-    const float d = softplusf_(v, &e);
-    return v != v ? v : d;                              // (fmaxf would drop a NaN)
+__device__ __forceinline__ f32x4 scan_delta4(f32x4 dt, f32x4 bias, int softplus) {
+    f32x4 v = dt + bias;
+    if (softplus)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = scan_softplus(v[i], nullptr);
+    return v;
 }
-__device__ __forceinline__ float scan_delta_grad(float dt, float bias, int softplus) {
-    if (!softplus) return 1.f;
-    return sigm(dt + bias);
+__device__ __forceinline__ f32x4 scan_delta4(f32x4 dt, f32x4 bias, int softplus, f32x4& slope) {
+    f32x4 v = dt + bias;
+    slope = f32x4{1.f, 1.f, 1.f, 1.f};
+    if (softplus)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float k;
+            v[i] = scan_softplus(v[i], &k);
+            slope[i] = k;
+        }
+    return v;
+}
+// (d, value) of four channels of one frame
+__device__ __forceinline__ void scan_stage(float2* at, f32x4 d, f32x4 v) {
+    reinterpret_cast<f32x4*>(at)[0] = f32x4{d[0], v[0], d[1], v[1]};
+    reinterpret_cast<f32x4*>(at)[1] = f32x4{d[2], v[2], d[3], v[3]};
 }
 
 // the 4 states of lane q, group g, of a [S] row (zeros behind the last)

@@ -41,21 +41,21 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
                                                        T* __restrict__ dx, T* __restrict__ ddt, T* __restrict__ dz, float* __restrict__ part_bc,
                                                        float* __restrict__ part_a, float* __restrict__ part_d,
                                                        const float* __restrict__ ends, const float* __restrict__ sums) {
-    __shared__ float2 dd[SCAN_TT][SCAN_CH];             // d, d x
-    __shared__ float go[SCAN_TT][SCAN_CH];
+    __shared__ __align__(16) float2 dd[SCAN_TT][SCAN_CH];             // d, d x
+    __shared__ __align__(16) float go[SCAN_TT][SCAN_CH];
     __shared__ __align__(16) float bs[SCAN_TT][NG * 16], cs[SCAN_TT][NG * 16];
-    __shared__ float us[SCAN_TT][SCAN_YP], ws[SCAN_TT][SCAN_YP], os[SCAN_TT][SCAN_YP];
+    __shared__ __align__(16) float us[SCAN_TT][SCAN_YP], ws[SCAN_TT][SCAN_YP], os[SCAN_TT][SCAN_YP];
     __shared__ float bc[4][SCAN_TT][NG * 32];           // per wave, frame: dB of the 16 NG states, dC
     const ScanBlock b = scan_block(a);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = tid & 3, cw = tid >> 2;
-    const int lr = tid >> 4, lc = (tid & 15) * 4, ln = b.cn - lc;
+    const int lr = tid >> 4, lc = (tid & 15) * 4, ln = b.cn - lc, ls = tid & 15;
     const int L = row_length(a.len, b.n, a.T);
     const bool on = cw < b.cn, svec = a.svec != 0;
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    const T* xp = (const T*)a.x + b.n * a.x_sn + b.c0 + lc;
-    const T* tp = (const T*)a.dt + b.n * a.dt_sn + b.c0 + lc;
-    const T* zp = a.z ? (const T*)a.z + b.n * a.z_sn + b.c0 + lc : nullptr;
-    const T* gp = dy + b.n * dy_sn + b.c0 + lc;
+    const T* xp = (const T*)a.x + b.n * a.x_sn + b.c0;
+    const T* tp = (const T*)a.dt + b.n * a.dt_sn + b.c0;
+    const T* zp = a.z ? (const T*)a.z + b.n * a.z_sn + b.c0 : nullptr;
+    const T* gp = dy + b.n * dy_sn + b.c0;
     const T* bp = (const T*)a.B + b.n * a.B_sn + b.grp * a.B_sg;
     const T* cp = (const T*)a.C + b.n * a.C_sn + b.grp * a.C_sg;
     const int64_t srow = ((int64_t)b.n * a.Ch + b.c0 + cw) * a.S;
@@ -75,19 +75,19 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
 
     f32x4 xr, tr, zr = zero, gr, h0[NG];
     float br[NG], cr[NG];
-    auto load = [&](int tile) {
-        const int64_t t = (int64_t)tile * SCAN_TT + lr;
-        const int m = t < L ? ln : 0;
-        xr = load4n<T, VEC>(xp + t * a.x_st, m);
-        tr = load4n<T, VEC>(tp + t * a.dt_st, m);
-        if (zp) zr = load4n<T, VEC>(zp + t * a.z_st, m);
-        gr = load4n<T, VEC>(gp + t * dy_st, m);
+    const ScanCols<VEC> cols(lc, b.cn);
+    auto load = [&](int tile) {                                         // (a frame behind the row's end: its last one, dropped again below)
+        const int f = tile * SCAN_TT + lr;
+        const int64_t t = f < L ? f : L - 1;
+        xr = cols.get(xp + t * a.x_st);
+        tr = cols.get(tp + t * a.dt_st);
+        if (zp) zr = cols.get(zp + t * a.z_st);
+        gr = cols.get(gp + t * dy_st);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            const int s = g * 16 + (tid & 15);
-            const bool in = t < L && s < a.S;
-            br[g] = in ? (float)bp[t * a.B_st + s] : 0.f;
-            cr[g] = in ? (float)cp[t * a.C_st + s] : 0.f;
+            const int s = g * 16 + ls < a.S ? g * 16 + ls : 0;
+            br[g] = (float)bp[t * a.B_st + s];
+            cr[g] = (float)cp[t * a.C_st + s];
             h0[g] = on ? scan_states4(hsave + ((int64_t)tile * a.N * a.Ch) * a.S + srow, g * 16 + 4 * q, a.S, svec) : zero;
         }
     };
@@ -100,20 +100,28 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
     for (int k = tiles - 1; k >= k0; --k) {
         const int64_t t = (int64_t)k * SCAN_TT + lr;
         const bool live = t < L;
-        const f32x4 xe = xr, te = tr, ze = zr, ge = gr;
-        f32x4 de, oe;                                                   // d, go of this thread's elements
+        // this thread's elements: x, d, softplus', go, and what o is multiplied by for dz; zeros behind the end and beside the channels
+        f32x4 slope;
+        const f32x4 xe = cols.keep(xr, live), de = cols.keep(scan_delta4(tr, bias, a.softplus, slope), live);
+        f32x4 oe = gr, gz = zero;
+        if (zp) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            de[i] = live && i < ln ? scan_delta(te[i], bias[i], a.softplus) : 0.f;
-            oe[i] = zp ? ge[i] * (ze[i] * sigm(ze[i])) : ge[i];
-            dd[lr][lc + i] = make_float2(de[i], de[i] * xe[i]);
-            go[lr][lc + i] = oe[i];
+            for (int i = 0; i < 4; ++i) {
+                const float s = sigm(zr[i]);
+                oe[i] = gr[i] * (zr[i] * s);
+                gz[i] = gr[i] * (s * fmaf(zr[i], 1.f - s, 1.f));
+            }
+            gz = cols.keep(gz, live);
         }
+        oe = cols.keep(oe, live);
+        scan_stage(&dd[lr][lc], de, de * xe);
+        *reinterpret_cast<f32x4*>(&go[lr][lc]) = oe;
         f32x4 h[NG];
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            bs[lr][g * 16 + (tid & 15)] = br[g];
-            cs[lr][g * 16 + (tid & 15)] = cr[g];
+            const bool in = live && g * 16 + ls < a.S;
+            bs[lr][g * 16 + ls] = in ? br[g] : 0.f;
+            cs[lr][g * 16 + ls] = in ? cr[g] : 0.f;
             h[g] = h0[g];
         }
         if (k > k0) load(k - 1);
@@ -185,22 +193,17 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
         __syncthreads();
         if (t < a.T) {
             f32x4 vx, vt, vz;
+            const f32x4 u = *reinterpret_cast<const f32x4*>(&us[lr][lc]), w = *reinterpret_cast<const f32x4*>(&ws[lr][lc]);
+            const f32x4 o = *reinterpret_cast<const f32x4*>(&os[lr][lc]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float u = us[lr][lc + i];
-                vx[i] = fmaf(de[i], u, Dv[i] * oe[i]);
-                vt[i] = fmaf(ws[lr][lc + i], SCAN_LN2, xe[i] * u) * scan_delta_grad(te[i], bias[i], a.softplus);
-                if (zp) {
-                    const float s = sigm(ze[i]), o = fmaf(Dv[i], xe[i], os[lr][lc + i]);
-                    vz[i] = ge[i] * o * s * fmaf(ze[i], 1.f - s, 1.f);
-                }
-                if (live && i < ln) {
-                    dD[i] = fmaf(oe[i], xe[i], dD[i]);
-                    dbias[i] += vt[i];
-                } else {
-                    vx[i] = vt[i] = vz[i] = 0.f;
-                }
+                vx[i] = fmaf(de[i], u[i], Dv[i] * oe[i]);
+                vt[i] = fmaf(w[i], SCAN_LN2, xe[i] * u[i]) * slope[i];
+                vz[i] = gz[i] * fmaf(Dv[i], xe[i], o[i]);
+                dD[i] = fmaf(oe[i], xe[i], dD[i]);
             }
+            vt = cols.keep(vt, live);
+            dbias += vt;
             const int64_t at = t * orow + obase;
             store4n<T, VEC>(dx + at, vx, ln);
             store4n<T, VEC>(ddt + at, vt, ln);
@@ -244,23 +247,31 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
     }
 }
 
-// dB, dC [T,N,G,S] from the partial sums of the group's workgroups, frames behind a row's end zero
+// The sums that cross workgroups, in one launch: workgroups [0, nbc) form dB and dC [T,N,G,S] from the partial sums of the group's
+// workgroups (frames behind a row's end: zeros), the next `na` form dA, the rest dD and ddt_bias.
 template <class T>
-__global__ __launch_bounds__(256) void scan_bc_kernel(const float* __restrict__ part, int TT, int N, int G, int S, int nblk, const int* __restrict__ len,
-                                                      T* __restrict__ dB, T* __restrict__ dC) {
-    const int64_t total = (int64_t)TT * N * G * S;
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
-        const int64_t row = e / S;
-        const int s = (int)(e - row * S);
-        const int64_t tn = row / G;
-        const int n = (int)(tn % N);
-        float vb = 0.f, vc = 0.f;
-        if (tn / N < row_length(len, n, TT)) {
-            const float* p = part + row * nblk * 2 * S + s;
-            for (int i = 0; i < nblk; ++i) { vb += p[(int64_t)(2 * i) * S]; vc += p[(int64_t)(2 * i + 1) * S]; }
+__global__ __launch_bounds__(256) void scan_finish_kernel(ScanDev a, const float* __restrict__ bc, const float* __restrict__ pa, const float* __restrict__ pd,
+                                                          int P, int nbc, int na, T* __restrict__ dB, T* __restrict__ dC, ColMap ma, ColMap md) {
+    if ((int)blockIdx.x >= nbc + na) return sum_columns(pd, P, 2 * a.Ch, md, blockIdx.x - nbc - na);
+    if ((int)blockIdx.x >= nbc) return sum_columns(pa, P, a.Ch * a.S, ma, blockIdx.x - nbc);
+    const int S2 = 2 * a.S;
+    const int64_t total = (int64_t)a.T * a.N * a.G * S2;
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)nbc * 256) {
+        const int64_t row = e / S2;
+        const int j = (int)(e - row * S2);
+        const int64_t tn = row / a.G;
+        float v = 0.f;
+        if (tn / a.N < row_length(a.len, (int)(tn % a.N), a.T)) {
+            const float* p = bc + row * a.nbg * S2 + j;
+            int i = 0;
+            for (; i + 4 <= a.nbg; i += 4) {
+                const float p0 = p[(int64_t)i * S2], p1 = p[(int64_t)(i + 1) * S2], p2 = p[(int64_t)(i + 2) * S2], p3 = p[(int64_t)(i + 3) * S2];
+                v += (p0 + p1) + (p2 + p3);
+            }
+            for (; i < a.nbg; ++i) v += p[(int64_t)i * S2];
         }
-        dB[e] = (T)vb;
-        dC[e] = (T)vc;
+        if (j < a.S) dB[row * a.S + j] = (T)v;
+        else dC[row * a.S + j - a.S] = (T)v;
     }
 }
 
@@ -315,10 +326,11 @@ extern "C" int aas_ssm_scan_bwd(aasStream_t stream, const aasScan* d, const void
     const bool empty = d->T == 0 || d->N == 0;
     if (d->Ch == 0) return 0;
     AAS_CHECK(dA != nullptr, "%s: null pointer", who);
-    const BwdWs w = empty ? BwdWs{0, 0, 0, 0, 0, 0} : bwd_ws(d->T, d->N, d->Ch, d->S, d->G);
-    const ScanChunks ck = empty ? ScanChunks{0, 0} : bwd_chunks(d->T, d->N, d->Ch, d->G);
-    char* base = (char*)ws;
+    AAS_CHECK((int64_t)d->Ch * (d->S + 2) <= 0x7fffffff, "%s: Ch = %d too large", who, d->Ch);
     if (!empty) {
+        const BwdWs w = bwd_ws(d->T, d->N, d->Ch, d->S, d->G);
+        const ScanChunks ck = bwd_chunks(d->T, d->N, d->Ch, d->G);
+        char* base = (char*)ws;
         AAS_CHECK(dy && hsave && dx && ddt && dB && dC && ws && (dz || !d->z), "%s: null pointer", who);
         AAS_CHECK(aas_aligned(hsave, 16) && aas_aligned(ws, 16), "%s: hsave and ws must be 16-byte aligned", who);
         ScanDev a;
@@ -332,16 +344,16 @@ extern "C" int aas_ssm_scan_bwd(aasStream_t stream, const aasScan* d, const void
                                                  (float*)(base + w.a), (float*)(base + w.d), (float*)(base + w.ends),
                                                  (float*)(base + w.sums)));
         AAS_LAUNCH_CHECK(who);
-        const int64_t total = (int64_t)d->T * d->N * d->G * d->S;
-        const int blocks = (int)(total / 256 + 1 < 4096 ? total / 256 + 1 : 4096);
-        AAS_DT_SWITCH(d->dtype, E, hipLaunchKernelGGL(scan_bc_kernel<E>, dim3(blocks), dim3(256), 0, s, (const float*)(base + w.bc), d->T, d->N, d->G,
-                                                      d->S, a.nbg, d->len, (E*)dB, (E*)dC));
+        const ColMap ma = {{dA, nullptr, nullptr, nullptr}, {d->Ch * d->S, 0, 0, 0}, 0, 1};
+        const ColMap md = {{dD, ddt_bias, nullptr, nullptr}, {d->Ch, d->Ch, 0, 0}, 0, 2};
+        const int64_t want = ((int64_t)d->T * d->N * d->G * 2 * d->S + 255) / 256;
+        const int nbc = (int)(want < 8192 ? want : 8192), na = cdiv((int64_t)d->Ch * d->S, 16), nd = dD || ddt_bias ? cdiv(2 * (int64_t)d->Ch, 16) : 0;
+        AAS_DT_SWITCH(d->dtype, E, hipLaunchKernelGGL(scan_finish_kernel<E>, dim3(nbc + na + nd), dim3(256), 0, s, a, (const float*)(base + w.bc),
+                                                      (const float*)(base + w.a), (const float*)(base + w.d), d->N * ck.n, nbc, na, (E*)dB, (E*)dC, ma, md));
         AAS_LAUNCH_CHECK(who);
+        return 0;
     }
-    const int P = empty ? 0 : d->N * ck.n;
-    ColMap ma = {{dA, nullptr, nullptr, nullptr}, {d->Ch * d->S, 0, 0, 0}, 0, 1};
-    if (aas_sum_partials(s, (const float*)(base + w.a), P, d->Ch * d->S, ma, who)) return 2;
-    if (!dD && !ddt_bias) return 0;
-    ColMap md = {{dD, ddt_bias, nullptr, nullptr}, {d->Ch, d->Ch, 0, 0}, 0, 2};
-    return aas_sum_partials(s, (const float*)(base + w.d), P, 2 * d->Ch, md, who);
+    // no frames: the sums of nothing
+    const ColMap ma = {{dA, dD, ddt_bias, nullptr}, {d->Ch * d->S, d->Ch, d->Ch, 0}, 0, 3};
+    return aas_sum_partials(s, nullptr, 0, d->Ch * (d->S + 2), ma, who);
 }

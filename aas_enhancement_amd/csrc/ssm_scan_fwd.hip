@@ -6,17 +6,17 @@ namespace {
 template <class T, int NG, bool VEC>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanDev a, float* __restrict__ state, T* __restrict__ y, float* __restrict__ hsave,
                                                        const float* __restrict__ ends, const float* __restrict__ sums) {
-    __shared__ float2 dd[2][SCAN_TT][SCAN_CH];          // d, d x
+    __shared__ __align__(16) float2 dd[2][SCAN_TT][SCAN_CH];          // d, d x
     __shared__ __align__(16) float bs[2][SCAN_TT][NG * 16], cs[2][SCAN_TT][NG * 16];
-    __shared__ float ys[2][SCAN_TT][SCAN_YP];
+    __shared__ __align__(16) float ys[2][SCAN_TT][SCAN_YP];
     const ScanBlock b = scan_block(a);
     const int tid = threadIdx.x, q = tid & 3, cw = tid >> 2;            // scanning: lane q of channel cw
-    const int lr = tid >> 4, lc = (tid & 15) * 4, ln = b.cn - lc;       // loading: channels lc .. lc+3 of frame lr of the tile
+    const int lr = tid >> 4, lc = (tid & 15) * 4, ln = b.cn - lc, ls = tid & 15;   // loading: channels lc .. lc+3 of frame lr of the tile
     const int L = row_length(a.len, b.n, a.T);
     const bool on = cw < b.cn, svec = a.svec != 0;
-    const T* xp = (const T*)a.x + b.n * a.x_sn + b.c0 + lc;
-    const T* tp = (const T*)a.dt + b.n * a.dt_sn + b.c0 + lc;
-    const T* zp = a.z ? (const T*)a.z + b.n * a.z_sn + b.c0 + lc : nullptr;
+    const T* xp = (const T*)a.x + b.n * a.x_sn + b.c0;
+    const T* tp = (const T*)a.dt + b.n * a.dt_sn + b.c0;
+    const T* zp = a.z ? (const T*)a.z + b.n * a.z_sn + b.c0 : nullptr;
     const T* bp = (const T*)a.B + b.n * a.B_sn + b.grp * a.B_sg;
     const T* cp = (const T*)a.C + b.n * a.C_sn + b.grp * a.C_sg;
 
@@ -41,31 +41,30 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanDev a, float* __restr
 
     f32x4 xr, tr, zr, xe, ze;
     float br[NG], cr[NG];
-    auto load = [&](int tile) {
-        const int64_t t = (int64_t)tile * SCAN_TT + lr;
-        const int m = t < L ? ln : 0;
-        xr = load4n<T, VEC>(xp + t * a.x_st, m);
-        tr = load4n<T, VEC>(tp + t * a.dt_st, m);
-        if (zp) zr = load4n<T, VEC>(zp + t * a.z_st, m);
+    const ScanCols<VEC> cols(lc, b.cn);
+    auto load = [&](int tile) {                                         // (a frame behind the row's end: its last one, dropped again in stage)
+        const int f = tile * SCAN_TT + lr;
+        const int64_t t = f < L ? f : L - 1;
+        xr = cols.get(xp + t * a.x_st);
+        tr = cols.get(tp + t * a.dt_st);
+        if (zp) zr = cols.get(zp + t * a.z_st);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {                                  // one state of one frame per thread and group
-            const int s = g * 16 + (tid & 15);
-            const bool in = t < L && s < a.S;
-            br[g] = in ? (float)bp[t * a.B_st + s] : 0.f;
-            cr[g] = in ? (float)cp[t * a.C_st + s] : 0.f;
+            const int s = g * 16 + ls < a.S ? g * 16 + ls : 0;
+            br[g] = (float)bp[t * a.B_st + s];
+            cr[g] = (float)cp[t * a.C_st + s];
         }
     };
     auto stage = [&](int tile, int u) {
-        const bool live = tile * SCAN_TT + lr < L;                      // behind the row's end: d = 0 leaves the state as it is
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float d = live && i < ln ? scan_delta(tr[i], bias[i], a.softplus) : 0.f;
-            dd[u][lr][lc + i] = make_float2(d, d * xr[i]);
-        }
+        const bool live = tile * SCAN_TT + lr < L;                      // behind the end: d = 0 leaves the state as it is
+        const f32x4 d = cols.keep(scan_delta4(tr, bias, a.softplus), live);
+        xr = cols.keep(xr, live);
+        scan_stage(&dd[u][lr][lc], d, d * xr);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            bs[u][lr][g * 16 + (tid & 15)] = br[g];
-            cs[u][lr][g * 16 + (tid & 15)] = cr[g];
+            const bool in = live && g * 16 + ls < a.S;
+            bs[u][lr][g * 16 + ls] = in ? br[g] : 0.f;
+            cs[u][lr][g * 16 + ls] = in ? cr[g] : 0.f;
         }
     };
     const int all = (L + SCAN_TT - 1) / SCAN_TT, k0 = blockIdx.y * a.tiles_per_chunk;
@@ -109,22 +108,22 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanDev a, float* __restr
             }
             ys[u][t + q][cw] = keep;
         }
-        f32x4 xn = xr, zn = zr;
+        f32x4 xn = xe, zn = ze;
         if (k + 1 < tiles) {
             stage(k + 1, u ^ 1);
+            xn = xr;
+            zn = zr;
             if (k + 2 < tiles) load(k + 2);
         }
         __syncthreads();
         if (k * SCAN_TT + lr < a.T) {
-            f32x4 o;
-            const bool live = k * SCAN_TT + lr < L;
+            f32x4 o = *reinterpret_cast<const f32x4*>(&ys[u][lr][lc]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                o[i] = fmaf(Dv[i], xe[i], ys[u][lr][lc + i]);
+                o[i] = fmaf(Dv[i], xe[i], o[i]);
                 if (zp) o[i] *= ze[i] * sigm(ze[i]);
-                if (!live) o[i] = 0.f;
             }
-            store4n<T, VEC>(yp, o, ln);
+            store4n<T, VEC>(yp, cols.keep(o, k * SCAN_TT + lr < L), ln);
         }
         xe = xn;
         ze = zn;
