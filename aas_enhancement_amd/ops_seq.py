@@ -7,42 +7,70 @@ every sum are fp32.  `lengths` (int32 [N] on the device, values brought into [0,
 lies behind them is not read, its outputs and gradients are zero.  Every call launches on the current stream of its tensors' device,
 may be captured into a graph, and gives the same bits on every run.  Names stand in `ops`: `ops.ssm_scan(...)`.
 """
-import ctypes as _ct
 import functools
 import math
+import struct
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ._lib import check, lib, ptr, require_cuda
 
 _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # include/aas_hip.h: AAS_DT_*
 
 
-class _CScan(_ct.Structure):
-    """include/aas_hip.h: aasScan"""
-    _fields_ = ([(n, _ct.c_int) for n in ("size", "dtype", "T", "N", "Ch", "S", "G", "softplus")]
-                + [(n, _ct.c_void_p) for n in ("x", "dt", "z", "B", "C", "A", "D", "dt_bias", "len")]
-                + [(n, _ct.c_int64) for n in ("x_st", "x_sn", "dt_st", "dt_sn", "z_st", "z_sn", "B_st", "B_sn", "B_sg", "C_st", "C_sn", "C_sg")])
+_raw_stream = torch._C._cuda_getCurrentRawStream     # what torch.cuda.current_stream().cuda_stream ends in, without the object (3-6 us a call)
+_empty = torch.empty
+
+# include/aas_hip.h: aasScan, as packed bytes (a ctypes.Structure of 36 fields takes 3 us longer to fill)
+_SCAN_FIELDS = (["size", "dtype", "T", "N", "Ch", "S", "G", "softplus"], ["x", "dt", "z", "B", "C", "A", "D", "dt_bias", "len"],
+                ["x_st", "x_sn", "dt_st", "dt_sn", "z_st", "z_sn", "B_st", "B_sn", "B_sg", "C_st", "C_sn", "C_sg"])
+_SCAN = struct.Struct("@%di%dP%dq" % tuple(len(f) for f in _SCAN_FIELDS))
 
 
 def _on_device(fn):
     """Run with the device of the first argument current (a call on a tensor of another device than the current one)."""
     @functools.wraps(fn)
     def wrapped(x, *a, **k):
-        if isinstance(x, torch.Tensor) and x.is_cuda and x.device.index != torch.cuda.current_device():
+        if isinstance(x, torch.Tensor) and x.is_cuda and x.get_device() != torch.cuda.current_device():
             with torch.cuda.device(x.device):
                 return fn(x, *a, **k)
         return fn(x, *a, **k)
     return wrapped
 
 
-def _stream():
-    return torch.cuda.current_stream().cuda_stream
+def _stream(t):
+    return _raw_stream(t.get_device())
+
+
+class _NoSecond(torch.autograd.Function):
+    """Hands a gradient on and refuses to be differentiated."""
+
+    @staticmethod
+    def forward(ctx, g, *anchors):
+        return g.view_as(g)
+
+    @staticmethod
+    def backward(ctx, *g):
+        raise RuntimeError("the causal sequence operators have first derivatives only: cannot differentiate through their gradients")
+
+
+def _first_order(backward):
+    """The backward passes are kernels without gradients of their own.  A recorded pass (create_graph=True) hands out gradients that
+    refuse to be differentiated wherever they depend on something that wants a gradient."""
+    @functools.wraps(backward)
+    def wrapped(ctx, *g):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *g)
+        with torch.no_grad():
+            out = backward(ctx, *g)
+        anchors = [t for t in (*ctx.saved_tensors, *g) if t is not None and t.requires_grad]
+        one = lambda o: o if o is None or not anchors else _NoSecond.apply(o, *anchors)   # noqa: E731
+        return tuple(one(o) for o in out)
+    return wrapped
 
 
 def _ws(nbytes, dev):
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    return _empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
 
 
 def _bad(who, what):
@@ -51,6 +79,8 @@ def _bad(who, what):
 
 def _activation(who, name, t, like=None, shape=None):
     """Checks of one activation; its channels made contiguous."""
+    if like is not None and isinstance(t, torch.Tensor) and t.dtype is like.dtype and t.device == like.device and t.shape == shape and t.stride(-1) == 1:
+        return t
     if not isinstance(t, torch.Tensor):
         _bad(who, "%s must be a tensor, got %s" % (name, type(t).__name__))
     require_cuda(t)
@@ -65,8 +95,8 @@ def _activation(who, name, t, like=None, shape=None):
 
 def _param(who, name, t, like, shape):
     """An fp32 parameter of the given shape, contiguous; None stays None."""
-    if t is None:
-        return None
+    if t is None or (t.dtype is torch.float32 and t.device == like.device and t.shape == shape and t.is_contiguous()):
+        return t
     require_cuda(t)
     if t.dtype != torch.float32 or t.device != like.device or tuple(t.shape) != tuple(shape):
         _bad(who, "%s must be fp32 %s on %s, got %s %s on %s" % (name, tuple(shape), like.device, t.dtype, tuple(t.shape), t.device))
@@ -74,8 +104,8 @@ def _param(who, name, t, like, shape):
 
 
 def _lengths(who, t, like, N):
-    if t is None:
-        return None
+    if t is None or (t.dtype is torch.int32 and t.shape == (N,) and t.device == like.device and t.is_contiguous()):
+        return t
     require_cuda(t)
     if t.dtype != torch.int32 or tuple(t.shape) != (N,) or t.device != like.device:
         _bad(who, "lengths must be int32 [%d] on %s, got %s %s on %s" % (N, like.device, t.dtype, tuple(t.shape), t.device))
@@ -100,6 +130,8 @@ def _wants_grad(*ts):
 
 def _rows(t):
     """-> (tensor, row pitch): the leading dimensions as uniformly spaced rows, copied where they are not."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
     pitch, seen = None, 1
     for size, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
         if size == 1:
@@ -116,8 +148,8 @@ def _rows(t):
 # ------------------------------------------------------------------------------------------------------------- causal convolution
 def _conv_fwd(x, weight, bias, silu, lengths, state):
     T, N, C = x.shape
-    y = torch.empty((T, N, C), device=x.device, dtype=x.dtype)
-    check(lib().aas_causal_conv1d_fwd(_stream(), _DT[x.dtype], T, N, C, weight.shape[1], x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(),
+    y = _empty((T, N, C), device=x.device, dtype=x.dtype)
+    check(lib().aas_causal_conv1d_fwd(_stream(x), _DT[x.dtype], T, N, C, weight.shape[1], x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(),
                                       ptr(bias), silu, ptr(lengths), ptr(state), y.data_ptr()), "aas_causal_conv1d_fwd")
     return y
 
@@ -130,7 +162,7 @@ class _CausalConv1d(torch.autograd.Function):
         return _conv_fwd(x, weight, bias, silu, lengths, None)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         x, weight, bias, lengths = ctx.saved_tensors
         T, N, C = x.shape
@@ -138,11 +170,11 @@ class _CausalConv1d(torch.autograd.Function):
         if dy.stride(-1) != 1:
             dy = dy.contiguous()
         need = ctx.needs_input_grad
-        dx = torch.empty((T, N, C), device=x.device, dtype=x.dtype) if need[0] else None
+        dx = _empty((T, N, C), device=x.device, dtype=x.dtype) if need[0] else None
         dw = torch.empty_like(weight) if need[1] else None
         db = torch.empty_like(bias) if need[2] else None
         ws = _ws(lib().aas_causal_conv1d_bwd_ws_bytes(T, N, C, K), x.device) if need[1] or need[2] else None
-        check(lib().aas_causal_conv1d_bwd(_stream(), _DT[x.dtype], T, N, C, K, x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(), ptr(bias),
+        check(lib().aas_causal_conv1d_bwd(_stream(x), _DT[x.dtype], T, N, C, K, x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(), ptr(bias),
                                           ctx.silu, ptr(lengths), dy.data_ptr(), dy.stride(0), dy.stride(1), ptr(dx), ptr(dw), ptr(db), ptr(ws)),
               "aas_causal_conv1d_bwd")
         return dx, dw, db, None, None
@@ -180,21 +212,22 @@ def causal_conv1d(x, weight, bias=None, activation="silu", lengths=None, state=N
 # ------------------------------------------------------------------------------------------------------------------------ the scan
 def _scan_desc(x, dt, A, B, C, D, z, dt_bias, softplus, lengths):
     T, N, Ch = x.shape
-    zs = (0, 0) if z is None else (z.stride(0), z.stride(1))
-    return _CScan(_ct.sizeof(_CScan), _DT[x.dtype], T, N, Ch, A.shape[1], B.shape[2], softplus,
-                  x.data_ptr(), dt.data_ptr(), ptr(z), B.data_ptr(), C.data_ptr(), A.data_ptr(), ptr(D), ptr(dt_bias), ptr(lengths),
-                  x.stride(0), x.stride(1), dt.stride(0), dt.stride(1), zs[0], zs[1], B.stride(0), B.stride(1), B.stride(2),
-                  C.stride(0), C.stride(1), C.stride(2))
+    xs, ds, bs, cs = x.stride(), dt.stride(), B.stride(), C.stride()
+    zs = xs if z is None else z.stride()
+    p = lambda t: 0 if t is None else t.data_ptr()     # noqa: E731
+    return _SCAN.pack(_SCAN.size, _DT[x.dtype], T, N, Ch, A.shape[1], B.shape[2], softplus,
+                      x.data_ptr(), dt.data_ptr(), p(z), B.data_ptr(), C.data_ptr(), A.data_ptr(), p(D), p(dt_bias), p(lengths),
+                      xs[0], xs[1], ds[0], ds[1], zs[0], zs[1], bs[0], bs[1], bs[2], cs[0], cs[1], cs[2])
 
 
 def _scan_fwd(x, dt, A, B, C, D, z, dt_bias, softplus, lengths, state, keep):
     T, N, Ch = x.shape
     S = A.shape[1]
-    y = torch.empty((T, N, Ch), device=x.device, dtype=x.dtype)
-    hsave = torch.empty(((T + 15) // 16, N, Ch, S), device=x.device, dtype=torch.float32) if keep else None
+    y = _empty((T, N, Ch), device=x.device, dtype=x.dtype)
+    hsave = _empty(((T + 15) // 16, N, Ch, S), device=x.device, dtype=torch.float32) if keep else None
     ws = _ws(lib().aas_ssm_scan_fwd_ws_bytes(T, N, Ch, S, B.shape[2]), x.device)
     d = _scan_desc(x, dt, A, B, C, D, z, dt_bias, softplus, lengths)
-    check(lib().aas_ssm_scan_fwd(_stream(), _ct.byref(d), ptr(state), y.data_ptr(), ptr(hsave), ptr(ws)), "aas_ssm_scan_fwd")
+    check(lib().aas_ssm_scan_fwd(_stream(x), d, ptr(state), y.data_ptr(), ptr(hsave), ptr(ws)), "aas_ssm_scan_fwd")
     return y, hsave
 
 
@@ -207,20 +240,21 @@ class _SsmScan(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         x, dt, A, B, C, D, z, dt_bias, lengths = ctx.saved_tensors
         T, N, Ch = x.shape
         S, G = A.shape[1], B.shape[2]
         if dy.stride(-1) != 1:
             dy = dy.contiguous()
-        new = lambda t, shape: None if t is None else torch.empty(shape, device=t.device, dtype=t.dtype)   # noqa: E731
-        dx, ddt, dz = (new(t, (T, N, Ch)) for t in (x, dt, z))
-        dB, dC = (new(t, (T, N, G, S)) for t in (B, C))
-        dA, dD, dbias = (None if t is None else torch.empty_like(t) for t in (A, D, dt_bias))
+        dx, ddt = x.new_empty((T, N, Ch)), x.new_empty((T, N, Ch))
+        dz = None if z is None else x.new_empty((T, N, Ch))
+        dB, dC, dA = x.new_empty((T, N, G, S)), x.new_empty((T, N, G, S)), A.new_empty((Ch, S))
+        dD = None if D is None else A.new_empty((Ch,))
+        dbias = None if dt_bias is None else A.new_empty((Ch,))
         ws = _ws(lib().aas_ssm_scan_bwd_ws_bytes(T, N, Ch, S, G), x.device)
         d = _scan_desc(x, dt, A, B, C, D, z, dt_bias, ctx.softplus, lengths)
-        check(lib().aas_ssm_scan_bwd(_stream(), _ct.byref(d), dy.data_ptr(), dy.stride(0), dy.stride(1), ctx.hsave.data_ptr(), dx.data_ptr(),
+        check(lib().aas_ssm_scan_bwd(_stream(x), d, dy.data_ptr(), dy.stride(0), dy.stride(1), ctx.hsave.data_ptr(), dx.data_ptr(),
                                      ddt.data_ptr(), ptr(dz), dB.data_ptr(), dC.data_ptr(), dA.data_ptr(), ptr(dD), ptr(dbias), ptr(ws)),
               "aas_ssm_scan_bwd")
         return dx, ddt, dA, dB, dC, dD, dz, dbias, None, None
@@ -298,7 +332,7 @@ def _drop_args(who, x, p, seed, offset):
 
 def _dropout_call(x, drop, seed_dev, used):
     y = torch.empty_like(x)
-    check(lib().aas_dropout(_stream(), _DT[x.dtype], x.numel(), x.data_ptr(), y.data_ptr(), drop[0], drop[1], drop[2], ptr(seed_dev), ptr(used)),
+    check(lib().aas_dropout(_stream(x), _DT[x.dtype], x.numel(), x.data_ptr(), y.data_ptr(), drop[0], drop[1], drop[2], ptr(seed_dev), ptr(used)),
           "aas_dropout")
     return y
 
@@ -310,7 +344,7 @@ class _Dropout(torch.autograd.Function):
         return _dropout_call(x, drop, drop[3], drop[4])
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         return _dropout_call(dy.contiguous(), ctx.drop, ctx.drop[4], None), None
 
@@ -334,10 +368,10 @@ def _res_fwd(x, x_ld, residual, res_ld, weight, bias, scale, eps, layer, drop, w
     C = x.shape[-1]
     R = x.numel() // C
     rt = x.dtype if residual is None else residual.dtype
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    r = torch.empty(x.shape, device=x.device, dtype=rt) if want_r else None
-    stat = torch.empty((R, 2), device=x.device, dtype=torch.float32) if want_stat else None
-    check(lib().aas_residual_norm_fwd(_stream(), _DT[x.dtype], _DT[rt], R, C, x.data_ptr(), x_ld, ptr(residual), res_ld, ptr(weight), ptr(bias),
+    y = _empty(x.shape, device=x.device, dtype=x.dtype)
+    r = _empty(x.shape, device=x.device, dtype=rt) if want_r else None
+    stat = _empty((R, 2), device=x.device, dtype=torch.float32) if want_stat else None
+    check(lib().aas_residual_norm_fwd(_stream(x), _DT[x.dtype], _DT[rt], R, C, x.data_ptr(), x_ld, ptr(residual), res_ld, ptr(weight), ptr(bias),
                                       ptr(scale), eps, layer, drop[0], drop[1], drop[2], ptr(drop[3]), ptr(drop[4]), y.data_ptr(), ptr(r),
                                       ptr(stat)), "aas_residual_norm_fwd")
     return y, r, stat
@@ -356,11 +390,11 @@ def _res_bwd(ctx, dy, dr):
         else:
             g, ld = _rows(g if g.stride(-1) == 1 or C == 1 else g.contiguous())
             args += [g, ld]
-    dx = torch.empty(shape, device=dev, dtype=ctx.x_dtype) if need[0] else None
-    dres = torch.empty(shape, device=dev, dtype=kept.dtype) if need[1] else None
-    dw, db, ds = (torch.empty(C, device=dev, dtype=torch.float32) if n else None for n in need[2:5])
+    dx = _empty(shape, device=dev, dtype=ctx.x_dtype) if need[0] else None
+    dres = _empty(shape, device=dev, dtype=kept.dtype) if need[1] else None
+    dw, db, ds = (_empty(C, device=dev, dtype=torch.float32) if n else None for n in need[2:5])
     ws = _ws(lib().aas_residual_norm_bwd_ws_bytes(R, C), dev) if need[2] or need[3] or need[4] else None
-    check(lib().aas_residual_norm_bwd(_stream(), _DT[ctx.x_dtype], _DT[kept.dtype], R, C, ptr(args[0]), args[1], ptr(args[2]), args[3], kept.data_ptr(),
+    check(lib().aas_residual_norm_bwd(_stream(kept), _DT[ctx.x_dtype], _DT[kept.dtype], R, C, ptr(args[0]), args[1], ptr(args[2]), args[3], kept.data_ptr(),
                                       ctx.kept_ld, ptr(x), ctx.x_ld, ctx.stat.data_ptr(), ptr(weight), ptr(scale), ctx.layer, drop[0], drop[1],
                                       drop[2], ptr(drop[4]), ptr(dx), ptr(dres), ptr(dw), ptr(db), ptr(ds), ptr(ws)), "aas_residual_norm_bwd")
     return dx, dres, dw, db, ds, None, None, None
@@ -380,7 +414,7 @@ class _ResidualNorm(torch.autograd.Function):
         return y, r
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy, dr):
         if dy is None and dr is None:
             return (None,) * 8
@@ -439,8 +473,8 @@ def residual_norm(x, residual=None, weight=None, bias=None, scale=None, eps=1e-5
 
 def _gated_fwd(x, x_ld, gate, gate_ld, weight, eps, groups, norm_first):
     C = x.shape[-1]
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    check(lib().aas_gated_norm_fwd(_stream(), _DT[x.dtype], x.numel() // C, C, groups, x.data_ptr(), x_ld, gate.data_ptr(), gate_ld, ptr(weight), eps,
+    y = _empty(x.shape, device=x.device, dtype=x.dtype)
+    check(lib().aas_gated_norm_fwd(_stream(x), _DT[x.dtype], x.numel() // C, C, groups, x.data_ptr(), x_ld, gate.data_ptr(), gate_ld, ptr(weight), eps,
                                    norm_first, y.data_ptr()), "aas_gated_norm_fwd")
     return y
 
@@ -454,7 +488,7 @@ class _GatedNorm(torch.autograd.Function):
         return _gated_fwd(x, x_ld, gate, gate_ld, weight, eps, groups, norm_first)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         x, gate, weight = ctx.saved_tensors
         x_ld, gate_ld, eps, groups, norm_first = ctx.args
@@ -462,10 +496,10 @@ class _GatedNorm(torch.autograd.Function):
         R = x.numel() // C
         dy, dy_ld = _rows(dy if dy.stride(-1) == 1 or C == 1 else dy.contiguous())
         need = ctx.needs_input_grad
-        dx, dg = (torch.empty(x.shape, device=x.device, dtype=x.dtype) if n else None for n in need[:2])
+        dx, dg = (_empty(x.shape, device=x.device, dtype=x.dtype) if n else None for n in need[:2])
         dw = torch.empty_like(weight) if need[2] else None
         ws = _ws(lib().aas_gated_norm_bwd_ws_bytes(R, C, groups), x.device) if need[2] else None
-        check(lib().aas_gated_norm_bwd(_stream(), _DT[x.dtype], R, C, groups, dy.data_ptr(), dy_ld, x.data_ptr(), x_ld, gate.data_ptr(), gate_ld,
+        check(lib().aas_gated_norm_bwd(_stream(x), _DT[x.dtype], R, C, groups, dy.data_ptr(), dy_ld, x.data_ptr(), x_ld, gate.data_ptr(), gate_ld,
                                        ptr(weight), eps, norm_first, ptr(dx), ptr(dg), ptr(dw), ptr(ws)), "aas_gated_norm_bwd")
         return dx, dg, dw, None, None, None
 

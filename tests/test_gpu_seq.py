@@ -517,6 +517,23 @@ def test_block_streams_frame_by_frame(ops):
     assert float((cs - c1).abs().max()) <= 2e-6 * float(cs.abs().max()) and float((ss - s1).abs().max()) <= 2e-6 * float(ss.abs().max())
 
 
+def test_first_derivatives_only(ops):
+    """A recorded backward pass is fine as long as nobody differentiates through it."""
+    x = torch.randn(4, 2, 8, device="cuda", requires_grad=True)
+    w = torch.randn(8, 4, device="cuda", requires_grad=True)
+    A, B, one = torch.full((8, 4), -1.0, device="cuda"), torch.randn(4, 2, 4, device="cuda"), torch.ones(4, 2, 8, device="cuda")
+    for f in (lambda: ops.causal_conv1d(x, w), lambda: ops.gated_norm(x, x), lambda: ops.residual_norm(x, x)[0], lambda: ops.residual_norm(x)[0],
+              lambda: ops.ssm_scan(x, x, A, B, B)):
+        y = f()
+        plain, = torch.autograd.grad(y, x, one, retain_graph=True)
+        g, = torch.autograd.grad(y, x, one, create_graph=True)
+        assert torch.equal(g, plain)
+        with pytest.raises(RuntimeError, match="first derivatives only"):
+            (g * x).sum().backward()
+    g, = torch.autograd.grad(ops.dropout(x, 0.5, 1), x, one, create_graph=True)
+    assert not g.requires_grad                                                 # linear: its gradient depends on nothing
+
+
 def test_results_repeat_and_streams(ops):
     """The same bits on every run, also from another stream than the tensors were made on."""
     i = scan_inputs(70, 3, 132, 16, 1, torch.bfloat16)

@@ -69,7 +69,7 @@ def host_checks(monkeypatch):
     from aas_enhancement_amd import ops_seq
     monkeypatch.setattr(ops_seq, "require_cuda", lambda *t: None)
 
-    def no_launch():
+    def no_launch(*a):
         raise AssertionError("launched")
     monkeypatch.setattr(ops_seq, "_stream", no_launch)
     return ops_seq
@@ -159,14 +159,11 @@ def test_c_entry_points_refuse_without_a_gpu():
     bad(L.aas_causal_conv1d_fwd(None, 0, 1, 1, 1, 4, None, 1, 1, one, None, 1, None, None, one), b"null")
     bad(L.aas_causal_conv1d_bwd(None, 0, -1, 1, 1, 4, one, 1, 1, one, None, 1, None, one, 1, 1, one, one, one, one), b"T = -1")
     bad(L.aas_causal_conv1d_bwd(None, 0, 1, 1, 1, 4, one, 1, 1, one, None, 1, None, one, 1, 1, one, one, one, None), b"null")
-    d = ops_seq._CScan(ctypes.sizeof(ops_seq._CScan), 0, 1, 1, 4, 16, 1, 1)
-    bad(L.aas_ssm_scan_fwd(None, ctypes.byref(d), None, one, None, None), b"null")
-    d.S = 65
-    bad(L.aas_ssm_scan_fwd(None, ctypes.byref(d), None, one, None, None), b"S = 65")
-    d.S, d.G = 16, 3
-    bad(L.aas_ssm_scan_bwd(None, ctypes.byref(d), one, 1, 1, one, one, one, None, one, one, one, None, None, one), b"no multiple")
-    d.size = 8
-    bad(L.aas_ssm_scan_fwd(None, ctypes.byref(d), None, one, None, None), b"aasScan.size")
+    desc = lambda S=16, G=1, size=ops_seq._SCAN.size: ops_seq._SCAN.pack(size, 0, 1, 1, 4, S, G, 1, *[0] * 21)   # noqa: E731
+    bad(L.aas_ssm_scan_fwd(None, desc(), None, one, None, None), b"null")
+    bad(L.aas_ssm_scan_fwd(None, desc(S=65), None, one, None, None), b"S = 65")
+    bad(L.aas_ssm_scan_bwd(None, desc(G=3), one, 1, 1, one, one, one, None, one, one, one, None, None, one), b"no multiple")
+    bad(L.aas_ssm_scan_fwd(None, desc(size=8), None, one, None, None), b"aasScan.size")
     bad(L.aas_residual_norm_fwd(None, 1, 2, 1, 8, one, 8, None, 0, None, None, None, 1e-5, 0, 0, 0, 0, None, None, one, one, None), b"r_dtype")
     bad(L.aas_residual_norm_fwd(None, 0, 0, 1, 16385, one, 8, None, 0, None, None, None, 1e-5, 0, 0, 0, 0, None, None, one, one, None), b"16384")
     bad(L.aas_residual_norm_fwd(None, 0, 0, 1, 8, one, 8, one, 8, None, None, None, 1e-5, 0, 0, 0, 0, None, None, one, None, None), b"r is wanted")
@@ -180,7 +177,7 @@ def test_c_entry_points_refuse_without_a_gpu():
 
 
 def test_scan_descriptor_matches_the_header():
-    """ops_seq._CScan has the fields of struct aasScan, in order."""
+    """ops_seq._SCAN packs the fields of struct aasScan, in order."""
     import os
     import re
     from aas_enhancement_amd import ops_seq
@@ -188,4 +185,4 @@ def test_scan_descriptor_matches_the_header():
     src = open(os.path.join(root, "include", "aas_hip.h")).read()
     body = re.sub(r"/\*.*?\*/", "", re.search(r"typedef struct aasScan \{(.*?)\} aasScan;", src, re.S).group(1), flags=re.S)
     names = [n.strip().lstrip("*").strip() for line in body.split(";") for n in re.sub(r"^\s*(const\s+)?(int64_t|int|void|float)\b", "", line).split(",") if n.strip()]
-    assert names == [f[0] for f in ops_seq._CScan._fields_]
+    assert names == sum(ops_seq._SCAN_FIELDS, [])
