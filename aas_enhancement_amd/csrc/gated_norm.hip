@@ -6,51 +6,62 @@
 
 namespace {
 
-__device__ __forceinline__ float gate_of(float z, float& slope) {
-    const float s = sigm(z);
-    slope = s * fmaf(z, 1.f - s, 1.f);
-    return z * s;
-}
-
 template <class T, int TPR, int NV, bool VEC, bool FIRST>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void gated_fwd_kernel(int64_t rows, int C, int cg, int groups, const T* __restrict__ x, int64_t x_ld,
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void gated_fwd_kernel(int64_t rows, int C, int cg, const T* __restrict__ x, int64_t x_ld,
                                                                            const T* __restrict__ z, int64_t z_ld, const float* __restrict__ w, float eps,
                                                                            T* __restrict__ y) {
     constexpr int RPB = TPR == 64 ? 4 : 1;
     __shared__ float s[TPR / 64][2];
-    const int l = threadIdx.x % TPR;
-    const int64_t id = (int64_t)blockIdx.x * RPB + (RPB > 1 ? threadIdx.x / TPR : 0);
-    const int64_t row = id / groups;
-    const int base = (int)(id - row * groups) * cg;
-    if (row >= rows) return;
-    f32x4 v[NV], gt[NV];
-    float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * TPR + l) * 4, n = cg - c;
-        v[i] = load4n<T, VEC>(x + row * x_ld + base + c, n);
-        gt[i] = load4n<T, VEC>(z + row * z_ld + base + c, n);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            gt[i][j] *= sigm(gt[i][j]);
-            if (!FIRST) v[i][j] *= gt[i][j];
-            if (j >= n) v[i][j] = 0.f;
-            s1 = fmaf(v[i][j], v[i][j], s1);
-        }
+    const int l = threadIdx.x % TPR, base = blockIdx.y * cg;
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    const float inv = 1.f / (float)cg;
+    int64_t row = (int64_t)blockIdx.x * RPB + (RPB > 1 ? threadIdx.x / TPR : 0);
+    x += base;
+    z += base;
+    RowRaw<T, NV> xn, zn;
+    if (row < rows) {
+        xn.template load<TPR, VEC>(x + row * x_ld, cg, l);
+        zn.template load<TPR, VEC>(z + row * z_ld, cg, l);
     }
-    row_sum2<TPR>(s1, s2, s);
-    const float rstd = 1.f / sqrtf(s1 / (float)cg + eps);
+    for (; row < rows; row += step) {                 // (whole waves, and whole workgroups where a row is one's)
+        f32x4 v[NV], gt[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * TPR + l) * 4, n = cg - c;
-        const f32x4 wv = w ? load4n<float, VEC>(w + base + c, n) : f32x4{1.f, 1.f, 1.f, 1.f};
-        f32x4 o;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            o[j] = v[i][j] * rstd * wv[j];
-            if (FIRST) o[j] *= gt[i][j];
+        for (int i = 0; i < NV; ++i) {
+            v[i] = xn.get(i);
+            gt[i] = zn.get(i);
         }
-        store4n<T, VEC>(y + row * C + base + c, o, n);
+        const bool more = row + step < rows;
+        if (row_ahead<TPR, NV>() && more) {
+            xn.template load<TPR, VEC>(x + (row + step) * x_ld, cg, l);
+            zn.template load<TPR, VEC>(z + (row + step) * z_ld, cg, l);
+        }
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)                  // (beyond the row x and z are zeros, and so is everything made of them)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                gt[i][j] *= sigm(gt[i][j]);
+                if (!FIRST) v[i][j] *= gt[i][j];
+                s1 = fmaf(v[i][j], v[i][j], s1);
+            }
+        row_sum2<TPR>(s1, s2, s);
+        const float rstd = __builtin_amdgcn_rsqf(fmaf(s1, inv, eps));
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = row_col<TPR, NV>(i, l), n = cg - c;
+            const f32x4 wv = w ? load4n<float, VEC>(w + base + c, n) : f32x4{1.f, 1.f, 1.f, 1.f};
+            f32x4 o;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                o[j] = v[i][j] * rstd * wv[j];
+                if (FIRST) o[j] *= gt[i][j];
+            }
+            store4n<T, VEC>(y + row * C + base + c, o, n);
+        }
+        if (!row_ahead<TPR, NV>() && more) {
+            xn.template load<TPR, VEC>(x + (row + step) * x_ld, cg, l);
+            zn.template load<TPR, VEC>(z + (row + step) * z_ld, cg, l);
+        }
     }
 }
 
@@ -63,57 +74,70 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void gated_bwd_kernel(int64_
     __shared__ float s[TPR / 64][2];
     __shared__ __align__(16) float cols[TPR == 64 ? 4 * NV * 256 : 4];
     const int l = threadIdx.x % TPR, base = blockIdx.y * cg;           // a workgroup stays in one group: its threads own columns
+    const int64_t step = (int64_t)gridDim.x * RPB;
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f}, one = {1.f, 1.f, 1.f, 1.f};
     f32x4 aw[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) aw[i] = zero;
     const float inv = 1.f / (float)cg;
-    for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < rows; row0 += (int64_t)gridDim.x * RPB) {
-        const int64_t row = row0 + (RPB > 1 ? threadIdx.x / TPR : 0);
-        if (row >= rows) continue;
-        f32x4 xv[NV], zv[NV], gv[NV];
+    int64_t row = (int64_t)blockIdx.x * RPB + (RPB > 1 ? threadIdx.x / TPR : 0);
+    x += base;
+    z += base;
+    dy += base;
+    RowRaw<T, NV> xn, zn, gn;
+    auto load = [&](int64_t r) {
+        xn.template load<TPR, VEC>(x + r * x_ld, cg, l);
+        zn.template load<TPR, VEC>(z + r * z_ld, cg, l);
+        gn.template load<TPR, VEC>(dy + r * dy_ld, cg, l);
+    };
+    if (row < rows) load(row);
+    for (; row < rows; row += step) {
+        const RowRaw<T, NV> xv = xn, zv = zn, gv = gn;
+        if (row_ahead<TPR, NV>() && row + step < rows) load(row + step);
         float s1 = 0.f, s2 = 0.f;
+        f32x4 sg[NV];                                                  // sigmoid of the gate
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * TPR + l) * 4, n = cg - c;
-            xv[i] = load4n<T, VEC>(x + row * x_ld + base + c, n);
-            zv[i] = load4n<T, VEC>(z + row * z_ld + base + c, n);
-            gv[i] = load4n<T, VEC>(dy + row * dy_ld + base + c, n);
-            const f32x4 wv = w ? load4n<float, VEC>(w + base + c, n) : one;
+            const int c = row_col<TPR, NV>(i, l), n = cg - c;
+            const f32x4 wv = w ? load4n<float, VEC>(w + base + c, n) : one, xf = xv.get(i), zf = zv.get(i), gf = gv.get(i);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float gt = zv[i][j] * sigm(zv[i][j]);
-                const float v = j < n ? (FIRST ? xv[i][j] : xv[i][j] * gt) : 0.f;
-                const float g = FIRST ? gv[i][j] * wv[j] * gt : gv[i][j] * wv[j];
+                sg[i][j] = sigm(zf[j]);
+                const float gt = zf[j] * sg[i][j];
+                const float v = FIRST ? xf[j] : xf[j] * gt;
+                const float g = FIRST ? gf[j] * wv[j] * gt : gf[j] * wv[j];
                 s1 = fmaf(v, v, s1);
                 s2 = fmaf(g, v, s2);
             }
         }
         row_sum2<TPR>(s1, s2, s);
-        const float rstd = 1.f / sqrtf(s1 * inv + eps), m = s2 * inv * rstd;   // mean(g hat)
+        const float rstd = __builtin_amdgcn_rsqf(fmaf(s1, inv, eps)), m = s2 * inv * rstd;   // m = mean(g hat)
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * TPR + l) * 4, n = cg - c;
-            const f32x4 wv = w ? load4n<float, VEC>(w + base + c, n) : one;
+            const int c = row_col<TPR, NV>(i, l), n = cg - c;
+            const f32x4 wv = w ? load4n<float, VEC>(w + base + c, n) : one, xf = xv.get(i), zf = zv.get(i), gf = gv.get(i);
             f32x4 ox, oz;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                float slope;
-                const float gt = gate_of(zv[i][j], slope);
-                const float hat = (FIRST ? xv[i][j] : xv[i][j] * gt) * rstd;
-                const float g = FIRST ? gv[i][j] * wv[j] * gt : gv[i][j] * wv[j];
+                const float sj = sg[i][j], gt = zf[j] * sj, slope = sj * fmaf(zf[j], 1.f - sj, 1.f);
+                const float hat = (FIRST ? xf[j] : xf[j] * gt) * rstd;
+                const float g = FIRST ? gf[j] * wv[j] * gt : gf[j] * wv[j];
                 const float dv = rstd * fmaf(-hat, m, g);
                 ox[j] = FIRST ? dv : dv * gt;
-                oz[j] = FIRST ? gv[i][j] * hat * wv[j] * slope : dv * xv[i][j] * slope;
-                if (j < n) aw[i][j] = fmaf(gv[i][j], FIRST ? hat * gt : hat, aw[i][j]);
+                oz[j] = FIRST ? gf[j] * hat * wv[j] * slope : dv * xf[j] * slope;
+                aw[i][j] = fmaf(gf[j], FIRST ? hat * gt : hat, aw[i][j]);
             }
             const int64_t at = row * C + base + c;
             if (dx) store4n<T, VEC>(dx + at, ox, n);
             if (dz) store4n<T, VEC>(dz + at, oz, n);
         }
+        if (!row_ahead<TPR, NV>() && row + step < rows) load(row + step);
     }
     if (part) put_columns<TPR, NV>(aw, part + (int64_t)blockIdx.x * C + base, cg, cols);
 }
+
+// workgroups a group: about eight a CU in all
+int gated_blocks(int64_t R, int C, int groups) { return norm_blocks(R, C / groups, groups >= 2048 ? 1 : 2048 / groups); }
 
 bool gated_args(const char* who, int dtype, int64_t R, int C, int groups) {
     if (!aas_dt_ok(dtype)) { aas_set_error("%s: dtype %d", who, dtype); return false; }
@@ -134,21 +158,16 @@ extern "C" int aas_gated_norm_fwd(aasStream_t stream, int dtype, int64_t R, int 
     const int es = aas_dt_size(dtype), cg = C / groups;
     const bool vec = cg % 4 == 0 && x_ld % 4 == 0 && gate_ld % 4 == 0 && aas_aligned(x, 4 * es) && aas_aligned(gate, 4 * es) && aas_aligned(y, 4 * es) &&
                      aas_aligned(weight, 16);
-    const unsigned grid = (unsigned)(cg <= 1024 ? (R * groups + 3) / 4 : R * groups);
+    const dim3 grid(gated_blocks(R, C, groups), groups);
 #define GO1(TPR, NV, VEC, FIRST)                                                                                                                  \
-    AAS_DT_SWITCH(dtype, E, hipLaunchKernelGGL((gated_fwd_kernel<E, TPR, NV, VEC, FIRST>), dim3(grid), dim3(TPR > 256 ? TPR : 256), 0,           \
-                                               (hipStream_t)stream, R, C, cg, groups, (const E*)x, x_ld, (const E*)gate, gate_ld, weight, eps, (E*)y))
+    AAS_DT_SWITCH(dtype, E, hipLaunchKernelGGL((gated_fwd_kernel<E, TPR, NV, VEC, FIRST>), grid, dim3(TPR > 256 ? TPR : 256), 0,                 \
+                                               (hipStream_t)stream, R, C, cg, (const E*)x, x_ld, (const E*)gate, gate_ld, weight, eps, (E*)y))
 #define GO(TPR, NV, VEC) if (norm_first) { GO1(TPR, NV, VEC, true) } else { GO1(TPR, NV, VEC, false) }
     AAS_ROW_SWITCH(cg, vec, GO);
 #undef GO
 #undef GO1
     AAS_LAUNCH_CHECK(who);
     return 0;
-}
-
-static int gated_blocks(int64_t R, int C, int groups) {              // workgroups per group: about 1024 in all
-    const int b = norm_bwd_blocks(R, C / groups), most = groups >= 1024 ? 1 : 1024 / groups;
-    return b < most ? b : most;
 }
 
 extern "C" size_t aas_gated_norm_bwd_ws_bytes(int64_t R, int C, int groups) {

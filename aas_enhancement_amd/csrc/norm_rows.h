@@ -1,10 +1,38 @@
 // Row norms of the causal block (residual_norm.hip, gated_norm.hip): one pass over the row, which stays in registers.  TPR threads
-// hold a row, thread l the columns 4 (i TPR + l) .. + 3 for i < NV.  Rows of up to 1024 columns are a wave each, four rows a workgroup, and
+// hold a row, each NV column quads: two neighbouring ones make one 16-byte access of a 16-bit type.  Rows of up to 1024 columns are a wave each, four rows a workgroup, and
 // need no barrier; longer ones are a workgroup's.
 #pragma once
 #include "seq_common.h"
 
 constexpr int NORM_MAX_C = 16384;
+
+// first column of quad i of thread l
+template <int TPR, int NV> __device__ __forceinline__ int row_col(int i, int l) {
+    return NV == 1 ? l * 4 : ((i >> 1) * TPR + l) * 8 + (i & 1) * 4;
+}
+
+// a row's share of one thread in its own type: what is read ahead for the next row
+template <class T, int NV> struct RowRaw {
+    vec_t<T, 4> q[NV];
+    template <int TPR, bool VEC> __device__ __forceinline__ void load(const T* row, int C, int l) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = row_col<TPR, NV>(i, l), n = C - c;
+            q[i] = vec_t<T, 4>{(T)0.f, (T)0.f, (T)0.f, (T)0.f};
+            if (VEC) {
+                if (n > 0) q[i] = *reinterpret_cast<const vec_t<T, 4>*>(row + c);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j < n) q[i][j] = row[c + j];
+            }
+        }
+    }
+    __device__ __forceinline__ f32x4 get(int i) const { return __builtin_convertvector(q[i], f32x4); }
+};
+// Rows go to resident workgroups in turn; with up to four quads a thread the next row is on its way while this one is worked on (more, or in a workgroup of 1024,
+// would not fit the registers of the backward passes).
+template <int TPR, int NV> constexpr bool row_ahead() { return NV <= 4 && TPR <= 256; }
 
 // sums of a and b over the row's threads, handed to all of them
 template <int TPR> __device__ __forceinline__ void row_sum2(float& a, float& b, float (*s)[2]) {
@@ -28,22 +56,23 @@ template <int TPR> __device__ __forceinline__ void row_sum2(float& a, float& b, 
     }
 }
 
-// the column sums acc[i] (columns 4 (i TPR + l)) of a workgroup's rows -> out[0 .. C); four rows a workgroup are joined through LDS
+// the column sums acc[i] (quad i) of a workgroup's rows -> out[0 .. C); four rows a workgroup are joined through LDS
 template <int TPR, int NV> __device__ __forceinline__ void put_columns(const f32x4* acc, float* out, int C, float* lds) {
     const int l = threadIdx.x % TPR, r = threadIdx.x / TPR;
     if (TPR == 64) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < NV; ++i) *reinterpret_cast<f32x4*>(lds + r * (NV * 256) + (i * 64 + l) * 4) = acc[i];
+        for (int i = 0; i < NV; ++i) *reinterpret_cast<f32x4*>(lds + r * (NV * 256) + row_col<TPR, NV>(i, l)) = acc[i];
         __syncthreads();
         for (int c = threadIdx.x; c < C; c += 256) out[c] = (lds[c] + lds[NV * 256 + c]) + (lds[2 * NV * 256 + c] + lds[3 * NV * 256 + c]);
     } else {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) store4n<float, false>(out + (i * TPR + l) * 4, acc[i], C - (i * TPR + l) * 4);
+        for (int i = 0; i < NV; ++i) store4n<float, false>(out + row_col<TPR, NV>(i, l), acc[i], C - row_col<TPR, NV>(i, l));
     }
 }
 
-// (threads a row, column quads a thread) by the number of columns; the element-wise (unaligned) form has the larger of each kind only
+// (threads a row, column quads a thread) by the number of columns.  The element-wise (unaligned) form has the larger of each kind only:
+// the quads it has beyond the row add zeros, so a row gives the same bits however it is aligned.
 #define AAS_ROW_SWITCH(C, vec, GO)                       \
     do {                                                 \
         if (vec) {                                       \
@@ -55,14 +84,15 @@ template <int TPR, int NV> __device__ __forceinline__ void put_columns(const f32
             else if ((C) <= 8192) { GO(256, 8, true); }  \
             else { GO(1024, 4, true); }                  \
         } else {                                         \
-            if ((C) <= 1024) { GO(64, 4, false); }       \
-            else if ((C) <= 4096) { GO(256, 4, false); } \
+            if ((C) <= 256) { GO(64, 1, false); }        \
+            else if ((C) <= 1024) { GO(64, 4, false); }  \
+            else if ((C) <= 8192) { GO(256, 8, false); } \
             else { GO(1024, 4, false); }                 \
         }                                                \
     } while (0)
 
-// workgroups of a backward pass, each of which leaves one partial row of the parameters' gradients
-static inline int norm_bwd_blocks(int64_t rows, int C) {
+// workgroups that share `rows` rows of C columns, at most `most`; in a backward pass each leaves one partial row of the parameters' gradients
+static inline int norm_blocks(int64_t rows, int C, int most) {
     const int64_t groups = C <= 1024 ? (rows + 3) / 4 : rows;
-    return (int)(groups < 512 ? (groups < 1 ? 1 : groups) : 512);
+    return (int)(groups < most ? (groups < 1 ? 1 : groups) : most);
 }

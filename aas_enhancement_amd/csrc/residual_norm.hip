@@ -20,66 +20,68 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_fwd_kernel(int
     constexpr int RPB = TPR == 64 ? 4 : 1;
     __shared__ float s[TPR / 64][2];
     const int l = threadIdx.x % TPR;
-    const int64_t row = (int64_t)blockIdx.x * RPB + (RPB > 1 ? threadIdx.x / TPR : 0);
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    const float inv = 1.f / (float)C;
+    const f32x4 one = {1.f, 1.f, 1.f, 1.f}, zero = {0.f, 0.f, 0.f, 0.f};
     const DropKey key = drop_key(dr.seed, dr.offset, dr.thr ? dr.d_seed : nullptr);
     if (used && blockIdx.x == 0 && threadIdx.x == 0) {
         used[0] = (int64_t)(((unsigned long long)key.k1 << 32) | key.k0);
         used[1] = (int64_t)key.off;
     }
-    if (row >= rows) return;                          // (a whole wave; only one-wave rows have more than one row a workgroup)
-    f32x4 v[NV];
-    float s1 = 0.f, s2 = 0.f;
+    int64_t row = (int64_t)blockIdx.x * RPB + (RPB > 1 ? threadIdx.x / TPR : 0);
+    RowRaw<T, NV> xn;
+    RowRaw<R, NV> rn;
+    auto load = [&](int64_t at) {
+        xn.template load<TPR, VEC>(x + at * x_ld, C, l);
+        if (res) rn.template load<TPR, VEC>(res + at * res_ld, C, l);
+    };
+    if (row < rows) load(row);
+    for (; row < rows; row += step) {                 // (whole waves, and whole workgroups where a row is one's)
+        f32x4 v[NV];
+        float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * TPR + l) * 4, n = C - c;
-        v[i] = load4n<T, VEC>(x + row * x_ld + c, n);
-        if (dr.thr && n > 0) v[i] = drop4<VEC>(v[i], row * C + c, key, dr.thr, dr.factor);
-        if (sc) {
-            const f32x4 k = load4n<float, VEC>(sc + c, n);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[i][j] *= k[j];
+        for (int i = 0; i < NV; ++i) {
+            const int c = row_col<TPR, NV>(i, l), n = C - c;
+            v[i] = xn.get(i);
+            if (dr.thr && n > 0) v[i] = drop4<VEC>(v[i], row * C + c, key, dr.thr, dr.factor);
+            if (sc) v[i] *= load4n<float, VEC>(sc + c, n);
+            if (res) v[i] += rn.get(i);
+            if (r_out) {
+                store4n<R, VEC>(r_out + row * C + c, v[i], n);
+                v[i] = __builtin_convertvector(__builtin_convertvector(v[i], vec_t<R, 4>), f32x4);
+            }
+            s1 += (v[i][0] + v[i][1]) + (v[i][2] + v[i][3]);
         }
-        if (res) {
-            const f32x4 k = load4n<R, VEC>(res + row * res_ld + c, n);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[i][j] += k[j];
+        if (row_ahead<TPR, NV>() && row + step < rows) load(row + step);
+        float mean = 0.f;
+        if (layer) {
+            row_sum2<TPR>(s1, s2, s);
+            mean = s1 * inv;
         }
-        if (r_out) {
-            store4n<R, VEC>(r_out + row * C + c, v[i], n);
+        s1 = s2 = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[i][j] = (float)(R)v[i][j];
-        }
-        if (n <= 0) v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        s1 += (v[i][0] + v[i][1]) + (v[i][2] + v[i][3]);
-    }
-    float mean = 0.f;
-    if (layer) {
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {             // the mean is taken off first: no difference of large squares
+                v[i][j] = row_col<TPR, NV>(i, l) + j < C ? v[i][j] - mean : 0.f;
+                s1 = fmaf(v[i][j], v[i][j], s1);
+            }
         row_sum2<TPR>(s1, s2, s);
-        mean = s1 / (float)C;
-    }
-    s1 = s2 = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {                 // the mean is taken off first: no difference of large squares
-            v[i][j] = (i * TPR + l) * 4 + j < C ? v[i][j] - mean : 0.f;
-            s1 = fmaf(v[i][j], v[i][j], s1);
+        const float rstd = __builtin_amdgcn_rsqf(fmaf(s1, inv, eps));
+        if (stat && l == 0) {
+            stat[2 * row] = mean;
+            stat[2 * row + 1] = rstd;
         }
-    row_sum2<TPR>(s1, s2, s);
-    const float rstd = 1.f / sqrtf(s1 / (float)C + eps);
-    if (stat && l == 0) {
-        stat[2 * row] = mean;
-        stat[2 * row + 1] = rstd;
-    }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * TPR + l) * 4, n = C - c;
-        f32x4 o;
-        const f32x4 one = {1.f, 1.f, 1.f, 1.f}, zero = {0.f, 0.f, 0.f, 0.f};
-        const f32x4 wv = w ? load4n<float, VEC>(w + c, n) : one, bv = b ? load4n<float, VEC>(b + c, n) : zero;
+        for (int i = 0; i < NV; ++i) {
+            const int c = row_col<TPR, NV>(i, l), n = C - c;
+            f32x4 o;
+            const f32x4 wv = w ? load4n<float, VEC>(w + c, n) : one, bv = b ? load4n<float, VEC>(b + c, n) : zero;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = fmaf(v[i][j] * rstd, wv[j], bv[j]);
-        store4n<T, VEC>(y + row * C + c, o, n);
+            for (int j = 0; j < 4; ++j) o[j] = fmaf(v[i][j] * rstd, wv[j], bv[j]);
+            store4n<T, VEC>(y + row * C + c, o, n);
+        }
+        if (!row_ahead<TPR, NV>() && row + step < rows) load(row + step);
     }
 }
 
@@ -94,27 +96,39 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_bwd_kernel(int
     __shared__ float s[TPR / 64][2];
     __shared__ __align__(16) float cols[TPR == 64 ? 4 * NV * 256 : 4];
     const int l = threadIdx.x % TPR;
+    const int64_t step = (int64_t)gridDim.x * RPB;
     const DropKey key = drop_key(dr.seed, dr.offset, dr.thr ? dr.d_seed : nullptr);
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f}, one = {1.f, 1.f, 1.f, 1.f};
     f32x4 aw[NV], ab[NV], as[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) aw[i] = ab[i] = as[i] = zero;
     const float inv = 1.f / (float)C;
-    for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < rows; row0 += (int64_t)gridDim.x * RPB) {
-        const int64_t row = row0 + (RPB > 1 ? threadIdx.x / TPR : 0);
-        if (row >= rows) continue;                    // (whole waves; a row's threads agree)
-        const float mean = stat[2 * row], rstd = stat[2 * row + 1];
+    int64_t row = (int64_t)blockIdx.x * RPB + (RPB > 1 ? threadIdx.x / TPR : 0);
+    RowRaw<T, NV> gn, xn;
+    RowRaw<R, NV> kn, dn;
+    float mean = 0.f, rstd = 0.f;
+    auto load = [&](int64_t at) {
+        if (dy) gn.template load<TPR, VEC>(dy + at * dy_ld, C, l);
+        kn.template load<TPR, VEC>(r + at * r_ld, C, l);
+        if (dro) dn.template load<TPR, VEC>(dro + at * dr_ld, C, l);
+        if (want_x) xn.template load<TPR, VEC>(x + at * x_ld, C, l);
+        mean = stat[2 * at];
+        rstd = stat[2 * at + 1];
+    };
+    if (row < rows) load(row);
+    for (; row < rows; row += step) {
         f32x4 g[NV], hat[NV];
         float s1 = 0.f, s2 = 0.f;
+        const float rs = rstd;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * TPR + l) * 4, n = C - c;
-            g[i] = dy ? load4n<T, VEC>(dy + row * dy_ld + c, n) : zero;
-            hat[i] = load4n<R, VEC>(r + row * r_ld + c, n);
+            const int c = row_col<TPR, NV>(i, l), n = C - c;
+            g[i] = dy ? gn.get(i) : zero;
+            hat[i] = kn.get(i);
             const f32x4 wv = w ? load4n<float, VEC>(w + c, n) : one;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                hat[i][j] = j < n ? (hat[i][j] - mean) * rstd : 0.f;
+                hat[i][j] = j < n ? (hat[i][j] - mean) * rs : 0.f;
                 aw[i][j] = fmaf(g[i][j], hat[i][j], aw[i][j]);
                 ab[i][j] += g[i][j];
                 g[i][j] *= wv[j];
@@ -122,32 +136,37 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_bwd_kernel(int
                 s2 += g[i][j];
             }
         }
+        const RowRaw<R, NV> dv = dn;
+        const RowRaw<T, NV> xv = xn;
+        if (row_ahead<TPR, NV>() && row + step < rows) load(row + step);
         row_sum2<TPR>(s1, s2, s);
         s1 *= inv;
         s2 = layer ? s2 * inv : 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * TPR + l) * 4, n = C - c;
-            f32x4 d = dro ? load4n<R, VEC>(dro + row * dr_ld + c, n) : zero;
+            const int c = row_col<TPR, NV>(i, l), n = C - c;
+            f32x4 d = dro ? dv.get(i) : zero;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) d[j] = fmaf(rstd, fmaf(-hat[i][j], s1, g[i][j] - s2), d[j]);
+            for (int j = 0; j < 4; ++j) d[j] = fmaf(rs, fmaf(-hat[i][j], s1, g[i][j] - s2), d[j]);
             if (dres) store4n<R, VEC>(dres + row * C + c, d, n);
-            if (want_x && n > 0) {
-                f32x4 xv = load4n<T, VEC>(x + row * x_ld + c, n);
-                if (dr.thr) xv = drop4<VEC>(xv, row * C + c, key, dr.thr, dr.factor);
+            if (n > 0) {
+                // the same bits keep or drop x (for dscale) and the gradient
+                f32x4 kept = one;
+                if (dr.thr) kept = drop4<VEC>(one, row * C + c, key, dr.thr, dr.factor);
+                if (want_x) {
+                    const f32x4 xf = xv.get(i);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) as[i][j] = j < n ? fmaf(d[j], xv[j], as[i][j]) : 0.f;
-            }
-            if (dx) {
-                if (sc) {
-                    const f32x4 k = load4n<float, VEC>(sc + c, n);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) d[j] *= k[j];
+                    for (int j = 0; j < 4; ++j) as[i][j] = j < n && kept[j] != 0.f ? fmaf(d[j], xf[j] * kept[j], as[i][j]) : as[i][j];
                 }
-                if (dr.thr && n > 0) d = drop4<VEC>(d, row * C + c, key, dr.thr, dr.factor);
-                store4n<T, VEC>(dx + row * C + c, d, n);
+                if (dx) {
+                    if (sc) d *= load4n<float, VEC>(sc + c, n);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) d[j] = kept[j] != 0.f ? d[j] * kept[j] : 0.f;
+                    store4n<T, VEC>(dx + row * C + c, d, n);
+                }
             }
         }
+        if (!row_ahead<TPR, NV>() && row + step < rows) load(row + step);
     }
     if (part) {
         float* p = part + (int64_t)blockIdx.x * 3 * C;
@@ -156,6 +175,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_bwd_kernel(int
         put_columns<TPR, NV>(as, p + 2 * C, C, cols);
     }
 }
+
+// workgroups of a backward pass: two a CU (their partial rows are 3 C sums each)
+int bwd_blocks(int64_t R, int C) { return norm_blocks(R, C, 512); }
 
 bool norm_args(const char* who, int dtype, int r_dtype, int64_t R, int C, int thr) {
     if (!aas_dt_ok(dtype) || !(r_dtype == dtype || r_dtype == AAS_DT_F32)) { aas_set_error("%s: dtype %d, r_dtype %d", who, dtype, r_dtype); return false; }
@@ -186,7 +208,7 @@ extern "C" int aas_residual_norm_fwd(aasStream_t stream, int dtype, int r_dtype,
     const bool vec = C % 4 == 0 && x_ld % 4 == 0 && (!residual || res_ld % 4 == 0) && aas_aligned(x, 4 * es) && aas_aligned(y, 4 * es) &&
                      aas_aligned(residual, 4 * rs) && aas_aligned(r, 4 * rs) && aas_aligned(weight, 16) && aas_aligned(bias, 16) && aas_aligned(scale, 16);
     const Drop dr = {(unsigned)thr, drop_factor(thr), seed, offset, d_seed};
-    const unsigned grid = (unsigned)(C <= 1024 ? (R + 3) / 4 : R);
+    const unsigned grid = (unsigned)norm_blocks(R, C, 2048);
 #define GO(TPR, NV, VEC)                                                                                                                       \
     AAS_NORM_TYPES(dtype, r_dtype, E, Q,                                                                                                       \
                    hipLaunchKernelGGL((residual_fwd_kernel<E, Q, TPR, NV, VEC>), dim3(grid), dim3(TPR > 256 ? TPR : 256), 0, (hipStream_t)stream, \
@@ -200,7 +222,7 @@ extern "C" int aas_residual_norm_fwd(aasStream_t stream, int dtype, int r_dtype,
 
 extern "C" size_t aas_residual_norm_bwd_ws_bytes(int64_t R, int C) {
     if (R <= 0 || C <= 0) return 0;
-    return (size_t)norm_bwd_blocks(R, C) * 3 * C * sizeof(float);
+    return (size_t)bwd_blocks(R, C) * 3 * C * sizeof(float);
 }
 
 extern "C" int aas_residual_norm_bwd(aasStream_t stream, int dtype, int r_dtype, int64_t R, int C, const void* dy, int64_t dy_ld, const void* dr_out,
@@ -219,7 +241,7 @@ extern "C" int aas_residual_norm_bwd(aasStream_t stream, int dtype, int r_dtype,
                          aas_aligned(dy, 4 * es) && aas_aligned(dr_out, 4 * rs) && aas_aligned(r, 4 * rs) && (!dscale || aas_aligned(x, 4 * es)) &&
                          aas_aligned(dx, 4 * es) && aas_aligned(dresidual, 4 * rs) && aas_aligned(weight, 16) && aas_aligned(scale, 16);
         const Drop dr = {(unsigned)thr, drop_factor(thr), seed, offset, d_seed};
-        P = norm_bwd_blocks(R, C);
+        P = bwd_blocks(R, C);
         float* part = params ? (float*)ws : nullptr;
 #define GO(TPR, NV, VEC)                                                                                                                           \
     AAS_NORM_TYPES(dtype, r_dtype, E, Q,                                                                                                           \

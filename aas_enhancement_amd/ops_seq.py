@@ -120,12 +120,16 @@ def _state(who, t, like, dtype, shape, given):
     if t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != like.device or not t.is_contiguous():
         _bad(who, "state must be contiguous %s %s on %s, got %s %s%s on %s"
              % (dtype, tuple(shape), like.device, t.dtype, tuple(t.shape), "" if t.is_contiguous() else " (strided)", t.device))
-    if torch.is_grad_enabled() and (t.requires_grad or any(g is not None and g.requires_grad for g in given)):
+    if _wants_grad(t, *given):
         _bad(who, "state= is for inference (under torch.no_grad() or on tensors without gradients): no gradient flows through it")
 
 
 def _wants_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _rows(t):
