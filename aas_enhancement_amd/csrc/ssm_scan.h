@@ -11,6 +11,7 @@
 
 constexpr int SCAN_CH = 64;      // channels per workgroup
 constexpr int SCAN_TT = 16;      // frames per tile
+constexpr int SCAN_HT = 8;       // frames between the states that the forward pass keeps for the backward pass
 constexpr int SCAN_YP = 80;      // pitch of a [16 frames][64 channels] tile that the scanning lanes write: 4 frames x 16 channels a wave, no two on one bank
 constexpr float SCAN_LOG2E = 1.4426950408889634f;
 constexpr float SCAN_LN2 = 0.6931471805599453f;

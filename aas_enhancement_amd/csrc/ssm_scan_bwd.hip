@@ -4,8 +4,9 @@
 //   u = sum_s g_s B_s,  w = sum_s q_s A_s:   dx = D go + d u,   dd = w + x u,   ddt = dd softplus',   dz = dy o (z sigmoid(z))',
 //   dA_s = sum_{t,n} q_s d,   dB_s = sum_c g_s d x,   dC_s = sum_c go h_s,   dD = sum go x,   ddt_bias = sum ddt.
 //
-// Tiles of 16 frames from the last to the first: a lane runs forward from the state that the forward pass kept in front of the tile,
-// holding p of the 16 frames in registers, then back through them.  dB and dC are sums over channels: eight values a lane (four
+// Tiles of 16 frames from the last to the first, in runs of 8: a lane goes forward from the state that the forward pass kept in front of
+// the run, holding a and p of its frames in registers, then back through them.  (States kept every 16 frames and the exponentials
+// formed twice was 289 us where this is XX, at 4096 x 4 x 1024; all 16 frames' a and p do not fit the registers.)  dB and dC are sums over channels: eight values a lane (four
 // states x {dB, dC}) over the 16 channels of a wave go by exchanges that halve the number of values with the number of lanes still to
 // add (lane halves, rows of 16, then within the row), then over the four waves through LDS, then - plain stores, no atomics - over the
 // workgroups by a second launch.
@@ -73,7 +74,8 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
     const f32x4 Dv = a.D ? load4n<float, false>(a.D + b.c0 + lc, ln) : zero;
     f32x4 dD = zero, dbias = zero;
 
-    f32x4 xr, tr, zr = zero, gr, h0[NG];
+    constexpr int HALVES = SCAN_TT / SCAN_HT;
+    f32x4 xr, tr, zr = zero, gr, h0[HALVES][NG];
     float br[NG], cr[NG];
     const ScanCols<VEC> cols(lc, b.cn);
     auto load = [&](int tile) {                                         // (a frame behind the row's end: its last one, dropped again below)
@@ -88,8 +90,12 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
             const int s = g * 16 + ls < a.S ? g * 16 + ls : 0;
             br[g] = (float)bp[t * a.B_st + s];
             cr[g] = (float)cp[t * a.C_st + s];
-            h0[g] = on ? scan_states4(hsave + ((int64_t)tile * a.N * a.Ch) * a.S + srow, g * 16 + 4 * q, a.S, svec) : zero;
         }
+#pragma unroll
+        for (int i = 0; i < HALVES; ++i)
+#pragma unroll
+            for (int g = 0; g < NG; ++g)                                // (kept also where the row ends inside the tile)
+                h0[i][g] = on ? scan_states4(hsave + ((int64_t)(tile * HALVES + i) * a.N * a.Ch) * a.S + srow, g * 16 + 4 * q, a.S, svec) : zero;
     };
     const int all = (L + SCAN_TT - 1) / SCAN_TT, k0 = chunk * a.tiles_per_chunk;
     const int k1 = k0 + a.tiles_per_chunk, tiles = k1 < all ? k1 : all;                       // tiles [k0, tiles) have frames, up to k1 are written
@@ -116,78 +122,85 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
         oe = cols.keep(oe, live);
         scan_stage(&dd[lr][lc], de, de * xe);
         *reinterpret_cast<f32x4*>(&go[lr][lc]) = oe;
-        f32x4 h[NG];
+        f32x4 h[HALVES][NG];
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             const bool in = live && g * 16 + ls < a.S;
             bs[lr][g * 16 + ls] = in ? br[g] : 0.f;
             cs[lr][g * 16 + ls] = in ? cr[g] : 0.f;
-            h[g] = h0[g];
+#pragma unroll
+            for (int i = 0; i < HALVES; ++i) h[i][g] = h0[i][g];
         }
         if (k > k0) load(k - 1);
         __syncthreads();
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            f32x4 p[SCAN_TT];                                           // a h[t-1]
-            float keep = 0.f;
+        for (int half = HALVES - 1; half >= 0; --half) {
+            constexpr int HT = SCAN_HT;
+            const int t0 = half * HT;
 #pragma unroll
-            for (int i = 0; i < SCAN_TT; ++i) {
-                const float2 d = dd[i][cw];
-                const f32x4 B = reinterpret_cast<const f32x4*>(bs[i])[g * 4 + q];
-                float acc = 0.f;
+            for (int g = 0; g < NG; ++g) {
+                f32x4 e[HT], p[HT], hh = h[half][g];                    // a, a h[t-1]
+                float keep = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    p[i][j] = __builtin_amdgcn_exp2f(d.x * A2[g][j]) * h[g][j];
-                    h[g][j] = fmaf(d.y, B[j], p[i][j]);
+                for (int i = 0; i < HT; ++i) {
+                    const float2 d = dd[t0 + i][cw];
+                    const f32x4 B = reinterpret_cast<const f32x4*>(bs[t0 + i])[g * 4 + q];
+                    float acc = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        e[i][j] = __builtin_amdgcn_exp2f(d.x * A2[g][j]);
+                        p[i][j] = e[i][j] * hh[j];
+                        hh[j] = fmaf(d.y, B[j], p[i][j]);
+                    }
+                    const f32x4 C = reinterpret_cast<const f32x4*>(cs[t0 + i])[g * 4 + q];   // (o, wanted for dz; without z it costs a few per cent)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc = fmaf(hh[j], C[j], acc);
+                    acc = quad_sum(acc);
+                    keep = q == (i & 3) ? acc : keep;
+                    if ((i & 3) == 3) {
+                        float* o = &os[t0 + (i & ~3) + q][cw];
+                        *o = g == 0 ? keep : *o + keep;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                const f32x4 C = reinterpret_cast<const f32x4*>(cs[i])[g * 4 + q];     // (o, wanted for dz; without z it costs a few per cent)
+                // B, C and d are read again (an address the compiler cannot match with the one above): kept from the run forward they would
+                // be 80 registers more
+                int ch = cw, sq = g * 4 + q;
+                asm volatile("" : "+v"(ch), "+v"(sq));
+                float ku = 0.f, kw = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc = fmaf(h[g][j], C[j], acc);
-                acc = quad_sum(acc);
-                keep = q == (i & 3) ? acc : keep;
-                if ((i & 3) == 3) {
-                    float* o = &os[(i & ~3) + q][cw];
-                    *o = g == 0 ? keep : *o + keep;
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            // B, d and the exponentials are read and formed again (an address the compiler cannot match with the one above): kept from the
-            // forward run, they would be 160 registers
-            int ch = cw, sq = g * 4 + q;
-            asm volatile("" : "+v"(ch), "+v"(sq));
-            float ku = 0.f, kw = 0.f;
+                for (int i = HT - 1; i >= 0; --i) {
+                    const float2 d = dd[t0 + i][ch];
+                    const float o = go[t0 + i][ch];
+                    const f32x4 B = reinterpret_cast<const f32x4*>(bs[t0 + i])[sq];
+                    const f32x4 C = reinterpret_cast<const f32x4*>(cs[t0 + i])[sq];
+                    float u = 0.f, w = 0.f, v[8];
 #pragma unroll
-            for (int i = SCAN_TT - 1; i >= 0; --i) {
-                const float2 d = dd[i][ch];
-                const float o = go[i][ch];
-                const f32x4 B = reinterpret_cast<const f32x4*>(bs[i])[sq];
-                const f32x4 C = reinterpret_cast<const f32x4*>(cs[i])[sq];
-                float u = 0.f, w = 0.f, v[8];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float gh = fmaf(C[j], o, carry[g][j]);
-                    v[4 + j] = o * fmaf(d.y, B[j], p[i][j]);
-                    v[j] = gh * d.y;
-                    u = fmaf(gh, B[j], u);
-                    const float r = gh * p[i][j];
-                    w = fmaf(r, A2[g][j], w);
-                    dA[g][j] = fmaf(r, d.x, dA[g][j]);
-                    carry[g][j] = gh * __builtin_amdgcn_exp2f(d.x * A2[g][j]);
+                    for (int j = 0; j < 4; ++j) {
+                        const float gh = fmaf(C[j], o, carry[g][j]);
+                        v[4 + j] = o * fmaf(d.y, B[j], p[i][j]);
+                        v[j] = gh * d.y;
+                        u = fmaf(gh, B[j], u);
+                        const float r = gh * p[i][j];
+                        w = fmaf(r, A2[g][j], w);
+                        dA[g][j] = fmaf(r, d.x, dA[g][j]);
+                        carry[g][j] = gh * e[i][j];
+                    }
+                    u = quad_sum(u);
+                    w = quad_sum(w);
+                    ku = q == (i & 3) ? u : ku;
+                    kw = q == (i & 3) ? w : kw;
+                    if ((i & 3) == 0) {
+                        float *pu = &us[t0 + i + q][cw], *pw = &ws[t0 + i + q][cw];
+                        *pu = g == 0 ? ku : *pu + ku;
+                        *pw = g == 0 ? kw : *pw + kw;
+                    }
+                    asm volatile("" : "+v"(dA[g][0]), "+v"(dA[g][1]), "+v"(dA[g][2]), "+v"(dA[g][3]));   // added up here, not products kept for later
+                    const float s = sum_channels8(v, (lane & 8) != 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                    // value (bit 5) + 2 (bit 4) is the state of the quad, bit 3 says dB or dC; the lanes that differ in bit 2 hold the same
+                    bc[wave][t0 + i][((lane & 8) ? NG * 16 : 0) + g * 16 + 4 * q + ((lane >> 5) & 1) + ((lane >> 3) & 2)] = s;
                 }
-                u = quad_sum(u);
-                w = quad_sum(w);
-                ku = q == (i & 3) ? u : ku;
-                kw = q == (i & 3) ? w : kw;
-                if ((i & 3) == 0) {
-                    float *pu = &us[i + q][cw], *pw = &ws[i + q][cw];
-                    *pu = g == 0 ? ku : *pu + ku;
-                    *pw = g == 0 ? kw : *pw + kw;
-                }
-                asm volatile("" : "+v"(dA[g][0]), "+v"(dA[g][1]), "+v"(dA[g][2]), "+v"(dA[g][3]));   // added up here, not 64 products kept for later
-                const float s = sum_channels8(v, (lane & 8) != 0);
-                __builtin_amdgcn_sched_barrier(0);
-                // value (bit 5) + 2 (bit 4) is the state of the quad, bit 3 says dB or dC; the lanes that differ in bit 2 hold the same
-                bc[wave][i][((lane & 8) ? NG * 16 : 0) + g * 16 + 4 * q + ((lane >> 5) & 1) + ((lane >> 3) & 2)] = s;
             }
         }
         __syncthreads();

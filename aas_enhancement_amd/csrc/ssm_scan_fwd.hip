@@ -81,13 +81,13 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanDev a, float* __restr
     }
     for (int k = k0; k < tiles; ++k, yp += ytile) {
         const int u = k & 1;
-        if (hsave && on) {
-            float* hp = hsave + ((int64_t)k * a.N * a.Ch) * a.S + srow;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) scan_put_states4(hp, g * 16 + 4 * q, a.S, svec, h[g]);
-        }
 #pragma unroll 1
         for (int t = 0; t < SCAN_TT; t += 4) {
+            if (hsave && on && t % SCAN_HT == 0) {
+                float* hp = hsave + ((int64_t)(k * (SCAN_TT / SCAN_HT) + t / SCAN_HT) * a.N * a.Ch) * a.S + srow;
+#pragma unroll
+                for (int g = 0; g < NG; ++g) scan_put_states4(hp, g * 16 + 4 * q, a.S, svec, h[g]);
+            }
             float keep = 0.f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {

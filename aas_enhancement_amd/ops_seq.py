@@ -228,7 +228,7 @@ def _scan_fwd(x, dt, A, B, C, D, z, dt_bias, softplus, lengths, state, keep):
     T, N, Ch = x.shape
     S = A.shape[1]
     y = _empty((T, N, Ch), device=x.device, dtype=x.dtype)
-    hsave = _empty(((T + 15) // 16, N, Ch, S), device=x.device, dtype=torch.float32) if keep else None
+    hsave = _empty((2 * ((T + 15) // 16), N, Ch, S), device=x.device, dtype=torch.float32) if keep else None
     ws = _ws(lib().aas_ssm_scan_fwd_ws_bytes(T, N, Ch, S, B.shape[2]), x.device)
     d = _scan_desc(x, dt, A, B, C, D, z, dt_bias, softplus, lengths)
     check(lib().aas_ssm_scan_fwd(_stream(x), d, ptr(state), y.data_ptr(), ptr(hsave), ptr(ws)), "aas_ssm_scan_fwd")
@@ -272,7 +272,7 @@ def ssm_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, length
     x, dt, z [T, N, Ch]; B, C [T, N, S] or [T, N, G, S] (channel c reads group c // (Ch / G)); all of one type.  A fp32 [Ch, S], D and dt_bias
     fp32 [Ch].  state fp32 [N, Ch, S]: h in front of the first frame, replaced in place by h behind each row's last one, so that a
     prompt is read in one call and single frames (T = 1) go on from it (inference only).  Without it h starts at zero; gradients for
-    every tensor, the backward pass forming h again from the states kept in front of every 16th frame."""
+    every tensor, the backward pass forming h again from the states kept in front of every 8th frame."""
     who = "ssm_scan"
     x = _activation(who, "x", x)
     if x.dim() != 3:

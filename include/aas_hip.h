@@ -569,7 +569,7 @@ typedef struct aasScan {
     const int* len;
     int64_t x_st, x_sn, dt_st, dt_sn, z_st, z_sn, B_st, B_sn, B_sg, C_st, C_sn, C_sg;
 } aasScan;
-/* hsave (NULL unless a backward pass follows): fp32 [ceil(T/16)][N][Ch][S], receives the state in front of every 16th frame. */
+/* hsave (NULL unless a backward pass follows): fp32 [2 ceil(T/16)][N][Ch][S], receives the state in front of every 8th frame. */
 size_t aas_ssm_scan_fwd_ws_bytes(int T, int N, int Ch, int S, int G);
 int aas_ssm_scan_fwd(aasStream_t stream, const aasScan* d, float* state, void* y, float* hsave, void* ws);
 /* Gradients of the call without a state; hsave as the forward pass left it.  dx, ddt, dz [T,N,Ch]; dB, dC [T,N,G,S]; dA [Ch,S];
