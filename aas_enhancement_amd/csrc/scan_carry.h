@@ -1,7 +1,7 @@
 // First launch of a scan whose time axis is split (ssm_scan.h): per chunk k and channel the sum of d, and what the chunk leaves behind when
 // nothing comes in:
-//   forward, k = 0 .. nchunk-2:  h = exp(d A) h + d x B  from zero (chunk 0: from the given state) over the chunk's frames;
-//   REV,     k = nchunk-1 .. 1:  c = exp(d A) (c + go C), from the last frame to the first: the gradient of the state in front of the chunk.
+//   forward, all but the last:  h = exp(d A) h + d x B  from zero (chunk 0: from the given state) over the chunk's frames;
+//   REV,     all but the first: c = exp(d A) (c + go C), from the last frame to the first: the gradient of the state in front of the chunk.
 #pragma once
 #include "ssm_scan.h"
 
@@ -13,7 +13,7 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(ScanDev a, const float*
     __shared__ __align__(16) float2 dd[2][SCAN_TT][SCAN_CH];          // d, and d x (REV: go)
     __shared__ __align__(16) float bs[2][SCAN_TT][NG * 16];
     const ScanBlock b = scan_block(a);
-    const int k = blockIdx.y + (REV ? 1 : 0);
+    const int k = blockIdx.y + (REV ? a.fine : 0), len = a.tiles_per_chunk / a.fine;
     const int tid = threadIdx.x, q = tid & 3, cw = tid >> 2;
     const int lr = tid >> 4, lc = (tid & 15) * 4, ln = b.cn - lc, ls = tid & 15;
     const int L = row_length(a.len, b.n, a.T);
@@ -36,8 +36,8 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(ScanDev a, const float*
     const f32x4 bias = a.dt_bias ? load4n<float, false>(a.dt_bias + b.c0 + lc, ln) : zero;
     f32x4 tr, vr, zr = zero, sum = zero;
     float br[NG];
-    const int tiles = (L + SCAN_TT - 1) / SCAN_TT, t0 = k * a.tiles_per_chunk;
-    const int t1 = t0 + a.tiles_per_chunk < tiles ? t0 + a.tiles_per_chunk : tiles;
+    const int tiles = (L + SCAN_TT - 1) / SCAN_TT, t0 = k * len;
+    const int t1 = t0 + len < tiles ? t0 + len : tiles;
     auto tile_of = [&](int i) { return REV ? t1 - 1 - i : t0 + i; };
     const ScanCols<VEC> cols(lc, b.cn);
     auto load = [&](int tile) {                         // (a frame behind the row's end: its last one, dropped again in stage)
@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(ScanDev a, const float*
     if (!REV && state && on && k == 0)
 #pragma unroll
         for (int g = 0; g < NG; ++g)
-            scan_put_states4(ends + ((a.nchunk - 1) * rows + ch) * a.S, g * 16 + 4 * q, a.S, svec, scan_states4(state + ch * a.S, g * 16 + 4 * q, a.S, svec));
+            scan_put_states4(ends + (((int64_t)a.nchunk * a.fine - 1) * rows + ch) * a.S, g * 16 + 4 * q, a.S, svec, scan_states4(state + ch * a.S, g * 16 + 4 * q, a.S, svec));
     if (on)
 #pragma unroll
         for (int g = 0; g < NG; ++g) scan_put_states4(ends + (k * rows + ch) * a.S, g * 16 + 4 * q, a.S, svec, h[g]);
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(ScanDev a, const float*
 
 template <class T, bool REV>
 void launch_carry(hipStream_t s, const ScanDev& a, bool vec, const float* state, const void* dy, int64_t dy_st, int64_t dy_sn, float* ends, float* sums) {
-    const dim3 grid((unsigned)((int64_t)a.N * a.nbg * a.G), a.nchunk - 1);
+    const dim3 grid((unsigned)((int64_t)a.N * a.nbg * a.G), (a.nchunk - 1) * a.fine);
 #define AAS_GO(NG_)                                                                                                                               \
     do {                                                                                                                                          \
         if (vec) hipLaunchKernelGGL((scan_carry_kernel<T, NG_, true, REV>), grid, dim3(256), 0, s, a, state, (const T*)dy, dy_st, dy_sn, ends, sums);  \

@@ -20,6 +20,7 @@ struct ScanDev {                 // aasScan with the pointers' types left to the
     int T, N, Ch, S, G, softplus;
     int cpg, nbg;                // channels per group, workgroups per group
     int tiles_per_chunk, nchunk; // chunks of the time axis (1: none)
+    int fine;                    // chunks of the carry launch per chunk of the main one
     int svec;                    // rows of S fp32 states (A, the state) can be read four at a time
     const void *x, *dt, *z, *B, *C;
     const float *A, *D, *dt_bias;
@@ -33,9 +34,9 @@ struct ScanDev {                 // aasScan with the pointers' types left to the
 // each decayed by exp(A sum of d) of the chunks between, which every workgroup of the main launch folds for itself.  The decays are
 // formed once more than unsplit, so it pays only where the chip is far from full.
 struct ScanChunks { int n, tiles; };
-ScanChunks scan_chunks(int T, int N, int Ch, int G, int want_blocks);
+ScanChunks scan_chunks(int T, int N, int Ch, int G, int want_blocks, int fine);
 
-// h in front of chunk k (REV: the carry behind it) from the chunks' ends [nchunk][N][Ch][S] and sums of d [nchunk][N][Ch]
+// h in front of carry chunk k (REV: the carry behind it) from the chunks' ends [nchunk][N][Ch][S] and sums of d [nchunk][N][Ch]
 template <int NG, bool REV>
 __device__ __forceinline__ void scan_fold(f32x4 (&h)[NG], const f32x4 (&A2)[NG], const float* ends, const float* sums, int k, int nchunk, int64_t rows,
                                           int64_t ch, int S, int q, bool svec);

@@ -6,7 +6,7 @@
 //
 // Tiles of 16 frames from the last to the first, in runs of 8: a lane goes forward from the state that the forward pass kept in front of
 // the run, holding a and p of its frames in registers, then back through them.  (States kept every 16 frames and the exponentials
-// formed twice was 289 us where this is XX, at 4096 x 4 x 1024; all 16 frames' a and p do not fit the registers.)  dB and dC are sums over channels: eight values a lane (four
+// formed twice was 289 us where this is 275, at 4096 x 4 x 1024; all 16 frames' a and p do not fit the registers.)  dB and dC are sums over channels: eight values a lane (four
 // states x {dB, dC}) over the 16 channels of a wave go by exchanges that halve the number of values with the number of lanes still to
 // add (lane halves, rows of 16, then within the row), then over the four waves through LDS, then - plain stores, no atomics - over the
 // workgroups by a second launch.
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
     }
     const int chunk = blockIdx.y;
     if (on && chunk + 1 < a.nchunk)
-        scan_fold<NG, true>(carry, A2, ends, sums, chunk, a.nchunk, (int64_t)a.N * a.Ch, (int64_t)b.n * a.Ch + b.c0 + cw, a.S, q, svec);
+        scan_fold<NG, true>(carry, A2, ends, sums, chunk * a.fine + a.fine - 1, a.nchunk * a.fine, (int64_t)a.N * a.Ch, (int64_t)b.n * a.Ch + b.c0 + cw, a.S, q, svec);
     const f32x4 bias = a.dt_bias ? load4n<float, false>(a.dt_bias + b.c0 + lc, ln) : zero;
     const f32x4 Dv = a.D ? load4n<float, false>(a.D + b.c0 + lc, ln) : zero;
     f32x4 dD = zero, dbias = zero;
@@ -288,7 +288,10 @@ __global__ __launch_bounds__(256) void scan_finish_kernel(ScanDev a, const float
     }
 }
 
-ScanChunks bwd_chunks(int T, int N, int Ch, int G) { return scan_chunks(T, N, Ch, G, 512); }
+// Two workgroups a CU: the kernel's 220 registers leave room for no more.  The carry launch needs a third of them and takes chunks of half
+// the length (at 4096 x 4 x 1024: 71 us against 88 with the main launch's own).
+constexpr int FINE = 2;
+ScanChunks bwd_chunks(int T, int N, int Ch, int G) { return scan_chunks(T, N, Ch, G, 512, FINE); }
 
 struct BwdWs { size_t bc, a, d, ends, sums, total; };   // byte offsets
 BwdWs bwd_ws(int T, int N, int Ch, int S, int G) {
@@ -299,8 +302,8 @@ BwdWs bwd_ws(int T, int N, int Ch, int S, int G) {
     w.a = up((size_t)T * N * G * cdiv(Ch / G, SCAN_CH) * 2 * S * sizeof(float));
     w.d = w.a + up((size_t)n * N * Ch * S * sizeof(float));
     w.ends = w.d + up((size_t)n * N * 2 * Ch * sizeof(float));
-    w.sums = w.ends + (n > 1 ? up((size_t)n * N * Ch * S * sizeof(float)) : 0);
-    w.total = w.sums + (n > 1 ? up((size_t)n * N * Ch * sizeof(float)) : 0);
+    w.sums = w.ends + (n > 1 ? up((size_t)n * FINE * N * Ch * S * sizeof(float)) : 0);
+    w.total = w.sums + (n > 1 ? up((size_t)n * FINE * N * Ch * sizeof(float)) : 0);
     return w;
 }
 
@@ -350,6 +353,7 @@ extern "C" int aas_ssm_scan_bwd(aasStream_t stream, const aasScan* d, const void
         scan_dev(d, &a);
         a.nchunk = ck.n;
         a.tiles_per_chunk = ck.tiles;
+        a.fine = FINE;
         const int al = 4 * aas_dt_size(d->dtype);
         const bool vec = scan_vec(a, d->dtype) && dy_st % 4 == 0 && dy_sn % 4 == 0 && aas_aligned(dy, al) && aas_aligned(dx, al) && aas_aligned(ddt, al) &&
                          (!dz || aas_aligned(dz, al));

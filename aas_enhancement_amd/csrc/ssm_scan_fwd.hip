@@ -171,7 +171,7 @@ void scan_dev(const aasScan* d, ScanDev* a) {
     a->cpg = d->Ch / d->G;
     a->nbg = cdiv(a->cpg, SCAN_CH);
     a->tiles_per_chunk = scan_tiles(d->T);
-    a->nchunk = 1;                                      // (set by the launcher)
+    a->nchunk = a->fine = 1;                                      // (set by the launcher)
     a->svec = d->S % 4 == 0 && aas_aligned(d->A, 16);
     a->x = d->x; a->dt = d->dt; a->z = d->z; a->B = d->B; a->C = d->C;
     a->A = d->A; a->D = d->D; a->dt_bias = d->dt_bias; a->len = d->len;
@@ -187,7 +187,7 @@ bool scan_vec(const ScanDev& a, int dtype) {
            aas_aligned(a.dt, al) && (!a.z || (a.z_st % 4 == 0 && a.z_sn % 4 == 0 && aas_aligned(a.z, al)));
 }
 
-ScanChunks scan_chunks(int T, int N, int Ch, int G, int want_blocks) {
+ScanChunks scan_chunks(int T, int N, int Ch, int G, int want_blocks, int fine) {
     const int tiles = scan_tiles(T);
     const int64_t blocks = (int64_t)N * cdiv(Ch / G, SCAN_CH) * G;
     ScanChunks c = {1, tiles};
@@ -196,12 +196,12 @@ ScanChunks scan_chunks(int T, int N, int Ch, int G, int want_blocks) {
     if (n > 32) n = 32;
     if (n > tiles / 4) n = tiles / 4;                   // at least four tiles a chunk
     if (n < 3) return c;                                // (two chunks: the carry launch and half of the main one take as long as the whole)
-    c.tiles = cdiv(tiles, n);
+    c.tiles = cdiv(cdiv(tiles, n), fine) * fine;
     c.n = cdiv(tiles, c.tiles);
     return c;
 }
 
-static ScanChunks fwd_chunks(int T, int N, int Ch, int G) { return scan_chunks(T, N, Ch, G, 1024); }
+static ScanChunks fwd_chunks(int T, int N, int Ch, int G) { return scan_chunks(T, N, Ch, G, 1024, 1); }
 
 extern "C" size_t aas_ssm_scan_fwd_ws_bytes(int T, int N, int Ch, int S, int G) {
     if (T <= 0 || N <= 0 || Ch <= 0 || S <= 0 || G <= 0 || Ch % G) return 0;
