@@ -288,10 +288,10 @@ __global__ __launch_bounds__(256) void scan_finish_kernel(ScanDev a, const float
     }
 }
 
-// Two workgroups a CU: the kernel's 220 registers leave room for no more.  The carry launch needs a third of them and takes chunks of half
-// the length (at 4096 x 4 x 1024: 71 us against 88 with the main launch's own).
+// Two workgroups a CU are resident (220 registers); twice as many even out the rows' lengths.  The carry launch needs a third of the
+// registers and takes chunks of half the length (at 4096 x 4 x 1024: 71 us against 88 with the main launch's own).
 constexpr int FINE = 2;
-ScanChunks bwd_chunks(int T, int N, int Ch, int G) { return scan_chunks(T, N, Ch, G, 512, FINE); }
+ScanChunks bwd_chunks(int T, int N, int Ch, int G) { return scan_chunks(T, N, Ch, G, 1024, FINE); }
 
 struct BwdWs { size_t bc, a, d, ends, sums, total; };   // byte offsets
 BwdWs bwd_ws(int T, int N, int Ch, int S, int G) {
