@@ -11,6 +11,44 @@
 
 namespace {
 
+// taps of four channels, w[channel][K] -> wk[tap][channel]; whole quads by 16-byte loads where the row is aligned for them
+template <int K> __device__ __forceinline__ void load_taps(f32x4 (&wk)[K], const float* w, int cn) {
+    if (cn == 4 && ((uintptr_t)w & 15) == 0) {
+        f32x4 v[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = reinterpret_cast<const f32x4*>(w)[k];
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) wk[k][i] = v[(i * K + k) / 4][(i * K + k) % 4];
+    } else {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) wk[k][i] = i < cn ? w[i * K + k] : 0.f;
+    }
+}
+
+// win[1 .. K-1] = the frames t0-K+1 .. t0-1 of a row of L frames: from the state (zeros without one) where a row begins, zeros behind its
+// end.  No load waits for another: addresses are chosen and brought inside, what is not wanted is dropped behind the loads.
+template <class T, int K, bool VEC>
+__device__ __forceinline__ void load_window(f32x4 (&win)[K], const T* xp, int64_t x_st, const T* sp, int64_t C, int t0, int L, int cn) {
+    const T* at[K - 1];
+    bool keep[K - 1];
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) {
+        const int t = t0 - (K - 1) + k, r = t < L ? t : L - 1;
+        at[k] = t >= 0 ? xp + (int64_t)(r > 0 ? r : 0) * x_st : (sp ? sp + (int64_t)(t + K - 1) * C : xp);
+        keep[k] = t >= 0 ? t < L : sp != nullptr;
+    }
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) win[k + 1] = load4n<T, VEC>(at[k], cn);
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) win[k + 1][i] = keep[k] ? win[k + 1][i] : 0.f;
+}
+
 template <class T, int K, bool VEC>
 __global__ __launch_bounds__(256) void conv_fwd_kernel(int TT, int N, int C, int CV, int stretch, int nstretch, const T* __restrict__ x, int64_t x_st,
                                                        int64_t x_sn, const float* __restrict__ w, const float* __restrict__ bias, int silu,
@@ -27,19 +65,10 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(int TT, int N, int C, int
     T* sp = state ? state + (int64_t)n * (K - 1) * C + c : nullptr;
 
     f32x4 wk[K], b = load4n<float, false>(bias ? bias + c : nullptr, bias ? cn : 0);
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) wk[k][i] = i < cn ? w[(int64_t)(c + i) * K + k] : 0.f;
+    load_taps<K>(wk, w + (int64_t)c * K, cn);
 
     f32x4 win[K];                                     // win[K-1] is the newest frame
-#pragma unroll
-    for (int k = 0; k < K - 1; ++k) {                 // frames t0-K+1 .. t0-1 -> win[1 .. K-1] behind the first shift
-        const int t = t0 - (K - 1) + k;
-        win[k + 1] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (t >= 0) { if (t < L) win[k + 1] = load4n<T, VEC>(xp + t * x_st, cn); }
-        else if (sp) win[k + 1] = load4n<T, VEC>(sp + (int64_t)(t + K - 1) * C, cn);
-    }
+    load_window<T, K, VEC>(win, xp, x_st, sp, C, t0, L, cn);
     const int te = t1 < L ? t1 : L;
     T* yp = y + ((int64_t)t0 * N + n) * C + c;
     const int64_t ys = (int64_t)N * C;
@@ -60,15 +89,15 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(int TT, int N, int C, int
         store4n<T, VEC>(yp, p, cn);
     }
     for (; t < t1; ++t, yp += ys) store4n<T, VEC>(yp, f32x4{0.f, 0.f, 0.f, 0.f}, cn);
-    // The new state is the last K-1 of [old state, the row's frames].  Stretches other than the first read the state's frames only when
-    // they begin inside the first K-1 frames, and a call with a state and more than one stretch has longer ones (the host's rule), so
-    // the thread that owns the first stretch is the only reader and the only writer.
-    if (sp && part == 0 && L > 0) {
+    // The new state is the last K-1 of [old state, the row's frames]: the window, where one thread has walked the whole row.  Where
+    // several share it, the first one's thread is the only reader of the old state (the others begin behind frame K-1), so it writes.
+    if (sp && L > 0 && part == 0) {
         f32x4 next[K - 1];
 #pragma unroll
         for (int k = 0; k < K - 1; ++k) {
             const int src = L - (K - 1) + k;          // frame index; < 0: from the old state
-            next[k] = src >= 0 ? load4n<T, VEC>(xp + src * x_st, cn) : load4n<T, VEC>(sp + (int64_t)(src + K - 1) * C, cn);
+            next[k] = nstretch == 1 ? win[k + 1]
+                                    : (src >= 0 ? load4n<T, VEC>(xp + src * x_st, cn) : load4n<T, VEC>(sp + (int64_t)(src + K - 1) * C, cn));
         }
 #pragma unroll
         for (int k = 0; k < K - 1; ++k) store4n<T, VEC>(sp + (int64_t)k * C, next[k], cn);
@@ -95,31 +124,19 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(int TT, int N, int C, int
 
     f32x4 wk[K], dw[K], b = load4n<float, false>(bias ? bias + c : nullptr, bias ? cn : 0), db = zero;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        dw[k] = zero;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) wk[k][i] = i < cn ? w[(int64_t)(c + i) * K + k] : 0.f;
-    }
+    for (int k = 0; k < K; ++k) dw[k] = zero;
+    load_taps<K>(wk, w + (int64_t)c * K, cn);
     f32x4 win[K], dp[K];                              // x[t-K+1 .. t], dp[t-K+1 .. t]
 #pragma unroll
     for (int k = 0; k < K; ++k) dp[k] = zero;
-#pragma unroll
-    for (int k = 0; k < K - 1; ++k) {
-        const int t = t0 - (K - 1) + k;
-        win[k + 1] = (t >= 0 && t < L) ? load4n<T, VEC>(xp + t * x_st, cn) : zero;
-    }
+    load_window<T, K, VEC>(win, xp, x_st, nullptr, C, t0, L, cn);
     const int64_t ys = (int64_t)N * C;
     T* op = dx ? dx + ((int64_t)t0 * N + n) * C + c : nullptr;
-#pragma unroll 4
-    for (int t = t0; t < te + K - 1; ++t) {           // dx[t-K+1] is complete behind dp[t]; dp of the next stretch's first frames is formed again
+    // One frame: dp[t], its share of dw and dbias (mine), and dx[t-K+1], which is complete behind dp[t].
+    auto frame = [&](int t, f32x4 xv, f32x4 g, bool mine) {
 #pragma unroll
         for (int k = 0; k < K - 1; ++k) { win[k] = win[k + 1]; dp[k] = dp[k + 1]; }
-        win[K - 1] = zero;
-        f32x4 g = zero;
-        if (t < L) {
-            win[K - 1] = load4n<T, VEC>(xp + t * x_st, cn);
-            g = load4n<T, VEC>(gp + t * dy_st, cn);
-        }
+        win[K - 1] = xv;
         if (silu) {
             f32x4 p = b;
 #pragma unroll
@@ -133,7 +150,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(int TT, int N, int C, int
             }
         }
         dp[K - 1] = g;
-        if (t < te) {
+        if (mine) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) db[i] += g[i];
 #pragma unroll
@@ -150,9 +167,19 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(int TT, int N, int C, int
             store4n<T, VEC>(op, v, cn);
             op += ys;
         }
+    };
+    // The stretch's own frames, whose loads nothing holds back; up to K-1 frames of the next stretch, whose dp is formed again; behind the
+    // row's end zeros.
+    int t = t0;
+#pragma unroll 4
+    for (; t < te; ++t) frame(t, load4n<T, VEC>(xp + t * x_st, cn), load4n<T, VEC>(gp + t * dy_st, cn), true);
+    if (te > t0) {
+        const int tl = te + K - 1 < L ? te + K - 1 : L;
+        for (; t < tl; ++t) frame(t, load4n<T, VEC>(xp + t * x_st, cn), load4n<T, VEC>(gp + t * dy_st, cn), false);
+        for (; t < te + K - 1; ++t) frame(t, zero, zero, false);
     }
     if (op)
-        for (int t = te > t0 ? te : t0; t < t1; ++t, op += ys) store4n<T, VEC>(op, zero, cn);
+        for (t = te > t0 ? te : t0; t < t1; ++t, op += ys) store4n<T, VEC>(op, zero, cn);
     if (part_out) {                                   // one row of [K taps | bias] x C per (stretch, n)
         float* pp = part_out + rest * (int64_t)(K + 1) * C + c;
 #pragma unroll
@@ -165,21 +192,22 @@ __global__ __launch_bounds__(256) void sum_partials_kernel(const float* __restri
     sum_columns(part, P, M, map, blockIdx.x);
 }
 
-// Stretch of the time axis per thread: long enough that the K - 1 overlapping frames cost little, short enough that the launch has the
-// ~128 k threads that keep the memory system busy.
-int conv_stretch(int T, int64_t rows4) {
-    const int64_t want = 131072;
-    int64_t per = want / (rows4 > 0 ? rows4 : 1);
+// Stretch of the time axis per thread: short enough that the launch has the 262144 threads that keep the memory system busy (half as many:
+// 37 us instead of 28 forward at 4096 x 4 x 2048 in bf16), and at least `least` frames - 8 forward, where an overlap of K - 1 frames
+// mostly hits the cache (200 x 30 x 1000 in fp32: 12.7 us, 13.8 with 16), 16 backward, where each stretch leaves a partial row of K + 1 sums.
+constexpr int FWD_LEAST = 8, BWD_LEAST = 16;
+int conv_stretch(int T, int N, int C, int least) {
+    const int64_t rows4 = (int64_t)cdiv(C, 4) * N;
+    int64_t per = 262144 / (rows4 > 0 ? rows4 : 1);
     if (per < 1) per = 1;
-    int s = cdiv(T, per);
-    if (s < 16) s = 16;
-    return s;
+    const int s = cdiv(T, per);
+    return s < least ? least : s;
 }
 
 template <int K, bool VEC>
 void launch_fwd(hipStream_t s, int dtype, int T, int N, int C, const void* x, int64_t x_st, int64_t x_sn, const float* w, const float* b, int silu,
                 const int* len, void* state, void* y) {
-    const int CV = cdiv(C, 4), st = conv_stretch(T, (int64_t)CV * N), ns = cdiv(T, st);
+    const int CV = cdiv(C, 4), st = conv_stretch(T, N, C, FWD_LEAST), ns = cdiv(T, st);
     const int64_t threads = (int64_t)CV * N * ns;
     AAS_DT_SWITCH(dtype, E, hipLaunchKernelGGL((conv_fwd_kernel<E, K, VEC>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, T, N, C, CV, st, ns,
                                                (const E*)x, x_st, x_sn, w, b, silu, len, (E*)state, (E*)y));
@@ -187,7 +215,7 @@ void launch_fwd(hipStream_t s, int dtype, int T, int N, int C, const void* x, in
 template <int K, bool VEC>
 void launch_bwd(hipStream_t s, int dtype, int T, int N, int C, const void* x, int64_t x_st, int64_t x_sn, const float* w, const float* b, int silu,
                 const int* len, const void* dy, int64_t dy_st, int64_t dy_sn, void* dx, float* part) {
-    const int CV = cdiv(C, 4), st = conv_stretch(T, (int64_t)CV * N), ns = cdiv(T, st);
+    const int CV = cdiv(C, 4), st = conv_stretch(T, N, C, BWD_LEAST), ns = cdiv(T, st);
     const int64_t threads = (int64_t)CV * N * ns;
     AAS_DT_SWITCH(dtype, E, hipLaunchKernelGGL((conv_bwd_kernel<E, K, VEC>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, T, N, C, CV, st, ns,
                                                (const E*)x, x_st, x_sn, w, b, silu, len, (const E*)dy, dy_st, dy_sn, (E*)dx, part));
@@ -230,7 +258,7 @@ extern "C" int aas_causal_conv1d_fwd(aasStream_t stream, int dtype, int T, int N
 
 extern "C" size_t aas_causal_conv1d_bwd_ws_bytes(int T, int N, int C, int K) {
     if (T <= 0 || N <= 0 || C <= 0 || K < 2 || K > 4) return 0;
-    return (size_t)cdiv(T, conv_stretch(T, (int64_t)cdiv(C, 4) * N)) * N * (K + 1) * C * sizeof(float);
+    return (size_t)cdiv(T, conv_stretch(T, N, C, BWD_LEAST)) * N * (K + 1) * C * sizeof(float);
 }
 
 extern "C" int aas_causal_conv1d_bwd(aasStream_t stream, int dtype, int T, int N, int C, int K, const void* x, int64_t x_st, int64_t x_sn,
@@ -241,7 +269,7 @@ extern "C" int aas_causal_conv1d_bwd(aasStream_t stream, int dtype, int T, int N
     hipStream_t s = (hipStream_t)stream;
     const bool empty = T == 0 || N == 0, params = dweight || dbias;
     AAS_CHECK(empty || (x && weight && dy && (ws || !params)), "aas_causal_conv1d_bwd: null pointer");
-    const int P = empty ? 0 : cdiv(T, conv_stretch(T, (int64_t)cdiv(C, 4) * N)) * N;
+    const int P = empty ? 0 : cdiv(T, conv_stretch(T, N, C, BWD_LEAST)) * N;
     if (!empty) {
         const int es = aas_dt_size(dtype);
         const bool vec = C % 4 == 0 && x_st % 4 == 0 && x_sn % 4 == 0 && dy_st % 4 == 0 && dy_sn % 4 == 0 && aas_aligned(x, 4 * es) &&

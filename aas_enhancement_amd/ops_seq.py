@@ -229,7 +229,7 @@ def _scan_fwd(x, dt, A, B, C, D, z, dt_bias, softplus, lengths, state, keep):
     S = A.shape[1]
     y = _empty((T, N, Ch), device=x.device, dtype=x.dtype)
     hsave = _empty((2 * ((T + 15) // 16), N, Ch, S), device=x.device, dtype=torch.float32) if keep else None
-    ws = _ws(lib().aas_ssm_scan_fwd_ws_bytes(T, N, Ch, S, B.shape[2]), x.device)
+    ws = None if T == 1 else _ws(lib().aas_ssm_scan_fwd_ws_bytes(T, N, Ch, S, B.shape[2]), x.device)
     d = _scan_desc(x, dt, A, B, C, D, z, dt_bias, softplus, lengths)
     check(lib().aas_ssm_scan_fwd(_stream(x), d, ptr(state), y.data_ptr(), ptr(hsave), ptr(ws)), "aas_ssm_scan_fwd")
     return y, hsave
