@@ -105,83 +105,86 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(int TT, int N, int C, int
 }
 
 template <class T, int K, bool VEC>
-__global__ __launch_bounds__(256) void conv_bwd_kernel(int TT, int N, int C, int CV, int stretch, int nstretch, const T* __restrict__ x, int64_t x_st,
+__global__ __launch_bounds__(256, 4) void conv_bwd_kernel(int TT, int N, int C, int CV, int stretch, int nstretch, int lanes, const T* __restrict__ x, int64_t x_st,
                                                        int64_t x_sn, const float* __restrict__ w, const float* __restrict__ bias, int silu,
                                                        const int* __restrict__ len, const T* __restrict__ dy, int64_t dy_st, int64_t dy_sn,
                                                        T* __restrict__ dx, float* __restrict__ part_out) {
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int cv = (int)(id % CV);
-    const int64_t rest = id / CV;
-    const int n = (int)(rest % N), part = (int)(rest / N);
-    if (part >= nstretch) return;
+    const int64_t first = id / CV;
+    if (first >= lanes) return;
     const int c = cv * 4, cn = C - c < 4 ? C - c : 4;
-    const int L = row_length(len, n, TT);
-    const int t0 = part * stretch, t1 = t0 + stretch < TT ? t0 + stretch : TT;
-    const int te = t1 < L ? t1 : L;
-    const T* xp = x + n * x_sn + c;
-    const T* gp = dy + n * dy_sn + c;
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
     f32x4 wk[K], dw[K], b = load4n<float, false>(bias ? bias + c : nullptr, bias ? cn : 0), db = zero;
 #pragma unroll
     for (int k = 0; k < K; ++k) dw[k] = zero;
     load_taps<K>(wk, w + (int64_t)c * K, cn);
-    f32x4 win[K], dp[K];                              // x[t-K+1 .. t], dp[t-K+1 .. t]
-#pragma unroll
-    for (int k = 0; k < K; ++k) dp[k] = zero;
-    load_window<T, K, VEC>(win, xp, x_st, nullptr, C, t0, L, cn);
     const int64_t ys = (int64_t)N * C;
-    T* op = dx ? dx + ((int64_t)t0 * N + n) * C + c : nullptr;
-    // One frame: dp[t], its share of dw and dbias (mine), and dx[t-K+1], which is complete behind dp[t].
-    auto frame = [&](int t, f32x4 xv, f32x4 g, bool mine) {
+    // a stretch of one row; where there are more of them than `lanes` (many short rows) a thread takes several, one partial row for all
+    for (int64_t rest = first; rest < (int64_t)N * nstretch; rest += lanes) {
+        const int n = (int)(rest % N), part = (int)(rest / N);
+        const int L = row_length(len, n, TT);
+        const int t0 = part * stretch, t1 = t0 + stretch < TT ? t0 + stretch : TT;
+        const int te = t1 < L ? t1 : L;
+        const T* xp = x + n * x_sn + c;
+        const T* gp = dy + n * dy_sn + c;
+        f32x4 win[K], dp[K];                              // x[t-K+1 .. t], dp[t-K+1 .. t]
 #pragma unroll
-        for (int k = 0; k < K - 1; ++k) { win[k] = win[k + 1]; dp[k] = dp[k + 1]; }
-        win[K - 1] = xv;
-        if (silu) {
-            f32x4 p = b;
+        for (int k = 0; k < K; ++k) dp[k] = zero;
+        load_window<T, K, VEC>(win, xp, x_st, nullptr, C, t0, L, cn);
+        T* op = dx ? dx + ((int64_t)t0 * N + n) * C + c : nullptr;
+        // One frame: dp[t], its share of dw and dbias (mine), and dx[t-K+1], which is complete behind dp[t].
+        auto frame = [&](int t, f32x4 xv, f32x4 g, bool mine) {
 #pragma unroll
-            for (int k = 0; k < K; ++k)
+            for (int k = 0; k < K - 1; ++k) { win[k] = win[k + 1]; dp[k] = dp[k + 1]; }
+            win[K - 1] = xv;
+            if (silu) {
+                f32x4 p = b;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) p[i] = fmaf(wk[k][i], win[k][i], p[i]);
+                for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float s = sigm(p[i]);
-                g[i] *= s * fmaf(p[i], 1.f - s, 1.f);
+                    for (int i = 0; i < 4; ++i) p[i] = fmaf(wk[k][i], win[k][i], p[i]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float s = sigm(p[i]);
+                    g[i] *= s * fmaf(p[i], 1.f - s, 1.f);
+                }
             }
-        }
-        dp[K - 1] = g;
-        if (mine) {
+            dp[K - 1] = g;
+            if (mine) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) db[i] += g[i];
+                for (int i = 0; i < 4; ++i) db[i] += g[i];
 #pragma unroll
-            for (int k = 0; k < K; ++k)
+                for (int k = 0; k < K; ++k)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) dw[k][i] = fmaf(g[i], win[k][i], dw[k][i]);
-        }
-        if (op && t >= t0 + K - 1) {
-            f32x4 v = zero;                           // dp[0] is frame t-K+1: its own tap is the newest, w[K-1]
+                    for (int i = 0; i < 4; ++i) dw[k][i] = fmaf(g[i], win[k][i], dw[k][i]);
+            }
+            if (op && t >= t0 + K - 1) {
+                f32x4 v = zero;                           // dp[0] is frame t-K+1: its own tap is the newest, w[K-1]
 #pragma unroll
-            for (int k = 0; k < K; ++k)
+                for (int k = 0; k < K; ++k)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = fmaf(wk[K - 1 - k][i], dp[k][i], v[i]);
-            store4n<T, VEC>(op, v, cn);
-            op += ys;
-        }
-    };
-    // The stretch's own frames, whose loads nothing holds back; up to K-1 frames of the next stretch, whose dp is formed again; behind the
-    // row's end zeros.
-    int t = t0;
+                    for (int i = 0; i < 4; ++i) v[i] = fmaf(wk[K - 1 - k][i], dp[k][i], v[i]);
+                store4n<T, VEC>(op, v, cn);
+                op += ys;
+            }
+        };
+        // The stretch's own frames, whose loads nothing holds back; up to K-1 frames of the next stretch, whose dp is formed again; behind the
+        // row's end zeros.
+        int t = t0;
 #pragma unroll 4
-    for (; t < te; ++t) frame(t, load4n<T, VEC>(xp + t * x_st, cn), load4n<T, VEC>(gp + t * dy_st, cn), true);
-    if (te > t0) {
-        const int tl = te + K - 1 < L ? te + K - 1 : L;
-        for (; t < tl; ++t) frame(t, load4n<T, VEC>(xp + t * x_st, cn), load4n<T, VEC>(gp + t * dy_st, cn), false);
-        for (; t < te + K - 1; ++t) frame(t, zero, zero, false);
+        for (; t < te; ++t) frame(t, load4n<T, VEC>(xp + t * x_st, cn), load4n<T, VEC>(gp + t * dy_st, cn), true);
+        if (te > t0) {
+            const int tl = te + K - 1 < L ? te + K - 1 : L;
+            for (; t < tl; ++t) frame(t, load4n<T, VEC>(xp + t * x_st, cn), load4n<T, VEC>(gp + t * dy_st, cn), false);
+            for (; t < te + K - 1; ++t) frame(t, zero, zero, false);
+        }
+        if (op)
+            for (t = te > t0 ? te : t0; t < t1; ++t, op += ys) store4n<T, VEC>(op, zero, cn);
     }
-    if (op)
-        for (t = te > t0 ? te : t0; t < t1; ++t, op += ys) store4n<T, VEC>(op, zero, cn);
-    if (part_out) {                                   // one row of [K taps | bias] x C per (stretch, n)
-        float* pp = part_out + rest * (int64_t)(K + 1) * C + c;
+    if (part_out) {                                   // one row of [K taps | bias] x C per lane
+        float* pp = part_out + first * (int64_t)(K + 1) * C + c;
 #pragma unroll
         for (int k = 0; k < K; ++k) store4n<float, false>(pp + (int64_t)k * C, dw[k], cn);
         store4n<float, false>(pp + (int64_t)K * C, db, cn);
@@ -204,6 +207,12 @@ int conv_stretch(int T, int N, int C, int least) {
     return s < least ? least : s;
 }
 
+// partial rows of the backward pass: every (stretch, row) its own while there are at most 2048, or as many as make 524288 threads
+int conv_lanes(int T, int N, int C) {
+    const int64_t all = (int64_t)cdiv(T, conv_stretch(T, N, C, BWD_LEAST)) * N, most = 524288 / cdiv(C, 4);
+    return (int)(all < 2048 ? all : (all < most ? all : (most > 2048 ? most : 2048)));
+}
+
 template <int K, bool VEC>
 void launch_fwd(hipStream_t s, int dtype, int T, int N, int C, const void* x, int64_t x_st, int64_t x_sn, const float* w, const float* b, int silu,
                 const int* len, void* state, void* y) {
@@ -215,15 +224,15 @@ void launch_fwd(hipStream_t s, int dtype, int T, int N, int C, const void* x, in
 template <int K, bool VEC>
 void launch_bwd(hipStream_t s, int dtype, int T, int N, int C, const void* x, int64_t x_st, int64_t x_sn, const float* w, const float* b, int silu,
                 const int* len, const void* dy, int64_t dy_st, int64_t dy_sn, void* dx, float* part) {
-    const int CV = cdiv(C, 4), st = conv_stretch(T, N, C, BWD_LEAST), ns = cdiv(T, st);
-    const int64_t threads = (int64_t)CV * N * ns;
+    const int CV = cdiv(C, 4), st = conv_stretch(T, N, C, BWD_LEAST), ns = cdiv(T, st), lanes = conv_lanes(T, N, C);
+    const int64_t threads = (int64_t)CV * lanes;
     AAS_DT_SWITCH(dtype, E, hipLaunchKernelGGL((conv_bwd_kernel<E, K, VEC>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, T, N, C, CV, st, ns,
-                                               (const E*)x, x_st, x_sn, w, b, silu, len, (const E*)dy, dy_st, dy_sn, (E*)dx, part));
+                                               lanes, (const E*)x, x_st, x_sn, w, b, silu, len, (const E*)dy, dy_st, dy_sn, (E*)dx, part));
 }
 
 bool conv_args_ok(const char* who, int dtype, int T, int N, int C, int K) {
     if (!aas_dt_ok(dtype)) { aas_set_error("%s: dtype %d", who, dtype); return false; }
-    if (T < 0 || N < 0 || C < 0) { aas_set_error("%s: T = %d, N = %d, C = %d", who, T, N, C); return false; }
+    if (T < 0 || N < 0 || C < 0 || T > (1 << 30)) { aas_set_error("%s: T = %d, N = %d, C = %d", who, T, N, C); return false; }
     if (K < 2 || K > 4) { aas_set_error("%s: K = %d, must be 2, 3 or 4", who, K); return false; }
     if (C > (1 << 24) || (int64_t)N * C > ((int64_t)1 << 36)) { aas_set_error("%s: N = %d, C = %d too large", who, N, C); return false; }
     return true;
@@ -258,7 +267,7 @@ extern "C" int aas_causal_conv1d_fwd(aasStream_t stream, int dtype, int T, int N
 
 extern "C" size_t aas_causal_conv1d_bwd_ws_bytes(int T, int N, int C, int K) {
     if (T <= 0 || N <= 0 || C <= 0 || K < 2 || K > 4) return 0;
-    return (size_t)cdiv(T, conv_stretch(T, N, C, BWD_LEAST)) * N * (K + 1) * C * sizeof(float);
+    return (size_t)conv_lanes(T, N, C) * (K + 1) * C * sizeof(float);
 }
 
 extern "C" int aas_causal_conv1d_bwd(aasStream_t stream, int dtype, int T, int N, int C, int K, const void* x, int64_t x_st, int64_t x_sn,
@@ -269,7 +278,7 @@ extern "C" int aas_causal_conv1d_bwd(aasStream_t stream, int dtype, int T, int N
     hipStream_t s = (hipStream_t)stream;
     const bool empty = T == 0 || N == 0, params = dweight || dbias;
     AAS_CHECK(empty || (x && weight && dy && (ws || !params)), "aas_causal_conv1d_bwd: null pointer");
-    const int P = empty ? 0 : cdiv(T, conv_stretch(T, N, C, BWD_LEAST)) * N;
+    const int P = empty ? 0 : conv_lanes(T, N, C);
     if (!empty) {
         const int es = aas_dt_size(dtype);
         const bool vec = C % 4 == 0 && x_st % 4 == 0 && x_sn % 4 == 0 && dy_st % 4 == 0 && dy_sn % 4 == 0 && aas_aligned(x, 4 * es) &&

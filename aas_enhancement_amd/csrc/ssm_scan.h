@@ -87,7 +87,7 @@ template <bool VEC> struct ScanCols {
 // 1/3 and atanh(s) / s a polynomial in s^2 (Chebyshev interpolation, off by 4e-9), so d keeps full relative accuracy where e is tiny (d
 // of 1e-3 and below), which log(1 + e) formed in fp32 has not.  The exponential takes the rounding of v log2(e) along.
 __device__ __forceinline__ float scan_softplus(float v, float* slope) {
-    const float m = fabsf(v), p = m * SCAN_LOG2E;
+    const float a = fabsf(v), m = a > 200.f ? 200.f : a, p = m * SCAN_LOG2E;               // (e is 0 from 104 on; an infinite m would make NaN below)
     const float lost = fmaf(m, SCAN_LOG2E, -p) + m * 1.925963033500e-8f;                // m log2(e) - p
     float e = __builtin_amdgcn_exp2f(-p);
     e = fmaf(e, -SCAN_LN2 * lost, e);

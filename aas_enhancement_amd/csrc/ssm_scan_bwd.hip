@@ -161,7 +161,7 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
                         float* o = &os[t0 + (i & ~3) + q][cw];
                         *o = g == 0 ? keep : *o + keep;
                     }
-                    __builtin_amdgcn_sched_barrier(0);
+                    if ((i & 3) == 3) __builtin_amdgcn_sched_barrier(0);
                 }
                 // B, C and d are read again (an address the compiler cannot match with the one above): kept from the run forward they would
                 // be 80 registers more
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
                     }
                     asm volatile("" : "+v"(dA[g][0]), "+v"(dA[g][1]), "+v"(dA[g][2]), "+v"(dA[g][3]));   // added up here, not products kept for later
                     const float s = sum_channels8(v, (lane & 8) != 0);
-                    __builtin_amdgcn_sched_barrier(0);
+                    if ((i & 3) == 0) __builtin_amdgcn_sched_barrier(0);           // (reads no further ahead: registers)
                     // value (bit 5) + 2 (bit 4) is the state of the quad, bit 3 says dB or dC; the lanes that differ in bit 2 hold the same
                     bc[wave][t0 + i][((lane & 8) ? NG * 16 : 0) + g * 16 + 4 * q + ((lane >> 5) & 1) + ((lane >> 3) & 2)] = s;
                 }

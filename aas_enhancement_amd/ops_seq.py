@@ -124,6 +124,11 @@ def _state(who, t, like, dtype, shape, given):
         _bad(who, "state= is for inference (under torch.no_grad() or on tensors without gradients): no gradient flows through it")
 
 
+def _written(state):
+    if not state.is_inference():     # (tensors made under inference_mode have no version to raise)
+        torch.autograd.graph.increment_version(state)
+
+
 def _wants_grad(*ts):
     if torch.is_grad_enabled():
         for t in ts:
@@ -206,7 +211,7 @@ def causal_conv1d(x, weight, bias=None, activation="silu", lengths=None, state=N
     if state is not None:
         _state(who, state, x, x.dtype, (N, weight.shape[1] - 1, C), (x, weight, bias))
         y = _conv_fwd(x, weight, bias, silu, lengths, state)
-        torch.autograd.graph.increment_version(state)
+        _written(state)
         return y
     if _wants_grad(x, weight, bias):
         return _CausalConv1d.apply(x, weight, bias, silu, lengths)
@@ -272,7 +277,8 @@ def ssm_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, length
     x, dt, z [T, N, Ch]; B, C [T, N, S] or [T, N, G, S] (channel c reads group c // (Ch / G)); all of one type.  A fp32 [Ch, S], D and dt_bias
     fp32 [Ch].  state fp32 [N, Ch, S]: h in front of the first frame, replaced in place by h behind each row's last one, so that a
     prompt is read in one call and single frames (T = 1) go on from it (inference only).  Without it h starts at zero; gradients for
-    every tensor, the backward pass forming h again from the states kept in front of every 8th frame."""
+    every tensor, the backward pass forming h again from the states kept in front of every 8th frame (T N Ch S / 2 bytes, held from the
+    forward pass on: 8 bytes an element at 16 states)."""
     who = "ssm_scan"
     x = _activation(who, "x", x)
     if x.dim() != 3:
@@ -301,7 +307,7 @@ def ssm_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, length
     if state is not None:
         _state(who, state, x, torch.float32, (N, Ch, S), (x, dt, A, B, C, D, z, dt_bias))
         y = _scan_fwd(x, dt, A, B, C, D, z, dt_bias, softplus, lengths, state, False)[0]
-        torch.autograd.graph.increment_version(state)
+        _written(state)
         return y
     if _wants_grad(x, dt, A, B, C, D, z, dt_bias):
         return _SsmScan.apply(x, dt, A, B, C, D, z, dt_bias, softplus, lengths)

@@ -254,6 +254,44 @@ def test_scan_views_and_padding(ops):
     close("batch first", y, ref["y"], mag["y"], k)
 
 
+def test_scan_infinite_and_tiny_steps(ops):
+    """softplus at the ends of its range: +-inf, the largest and the smallest numbers; a NaN stays in its channel."""
+    v = torch.tensor([float("-inf"), -3e38, -120.0, -100.0, -20.0, -1e-30, 0.0, 1e-30, 30.0, 120.0])
+    T, Ch = 3, v.numel() + 1
+    dt = torch.zeros(T, 1, Ch)
+    dt[1, 0, :-1], dt[1, 0, -1] = v, float("nan")
+    x, B, C = torch.ones(T, 1, Ch), torch.ones(T, 1, 2), torch.ones(T, 1, 2)
+    A = torch.tensor([[-1.0, -0.5]]).repeat(Ch, 1)
+    y = ops.ssm_scan(dev(x), dev(dt), dev(A), dev(B), dev(C)).cpu()
+    ref = seq.scan(x, dt, A, B, C)["y"]
+    assert torch.isnan(y[1:, 0, -1]).all() and not torch.isnan(y[0]).any() and not torch.isnan(y[:, 0, :-1]).any()
+    close("y", y[:, :, :-1], ref[:, :, :-1], ref[:, :, :-1].abs() + 1, 200)
+    d = ops.ssm_scan(dev(x[:1]), dev(dt[1:2]), dev(A), dev(B[:1]), dev(C[:1]))[0, 0, :-1].cpu().double() / 2          # x = B = C = 1: y = 2 d
+    want = torch.logaddexp(v.double(), torch.zeros(10, dtype=torch.float64))
+    small = want > 1e-37                                                       # (below, the exponential is 0)
+    assert bool((((d - want) / want).abs()[small] < 8 * U * (1 + v.double().abs().clamp(max=120))[small]).all())
+
+
+def test_inference_mode_and_many_short_rows(ops):
+    with torch.inference_mode():
+        st, cs = torch.zeros(2, 8, 16, device="cuda"), torch.zeros(2, 3, 8, device="cuda")
+        x, B = torch.randn(1, 2, 8, device="cuda"), torch.randn(1, 2, 16, device="cuda")
+        ops.ssm_scan(ops.causal_conv1d(x, torch.ones(8, 4, device="cuda"), state=cs), x, -torch.ones(8, 16, device="cuda"), B, B, state=st)
+        assert bool(st.any()) and bool(cs.any())
+    x, w, b = torch.randn(3, 5000, 8), torch.randn(8, 3), torch.randn(8)
+    n = torch.randint(0, 4, (5000,), dtype=torch.int32)
+    big = torch.randn(2, 140000, 4)
+    for x, n in ((x, n), (big, None)):                                         # more rows than partial rows
+        ws, bs = w[:x.shape[2]], b[:x.shape[2]]
+        dy = torch.randn(x.shape)
+        a, ww, bb = leaves(x, ws, bs)
+        ops.causal_conv1d(a, ww, bb, lengths=dev(n)).backward(dev(dy))
+        ref, mag = seq.conv(x, ws, bs, lengths=n, dy=dy), seq.conv(x, ws, bs, lengths=n, dy=dy, mag=True)
+        close("dx", a.grad, ref["dx"], mag["dx"], 46)
+        close("dw", ww.grad, ref["dw"], mag["dw"], 60 + 3000)                  # chains: a thread's rows, then the partial rows by 16
+        close("db", bb.grad, ref["db"], mag["db"], 60 + 3000)
+
+
 def test_scan_prompt_then_frames(ops):
     """A prompt read into the state and single frames going on from it, against the whole in 64 bits; a length outside [0, T] is brought in."""
     i = scan_inputs(60, 2, 40, 16, 1, torch.float32, lengths=False)
