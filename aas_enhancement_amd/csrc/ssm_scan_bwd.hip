@@ -6,7 +6,9 @@
 //
 // Tiles of 16 frames from the last to the first, in runs of 8: a lane goes forward from the state that the forward pass kept in front of
 // the run, holding a and p of its frames in registers, then back through them.  (States kept every 16 frames and the exponentials
-// formed twice was 289 us where this is 275, at 4096 x 4 x 1024; all 16 frames' a and p do not fit the registers.)  dB and dC are sums over channels: eight values a lane (four
+// formed twice was 289 us where this was 275, at 4096 x 4 x 1024 in bf16; now 263, at 200 x 30 x 1000 in fp32 91.  All 16 frames' a and p
+// do not fit the registers.)  Bound by instruction issue (105 a frame and wave, VALU active in 77 % of the busy cycles) at two waves a
+// SIMD; held to three by launch bounds it spills: 561 us.  dB and dC are sums over channels: eight values a lane (four
 // states x {dB, dC}) over the 16 channels of a wave go by exchanges that halve the number of values with the number of lanes still to
 // add (lane halves, rows of 16, then within the row), then over the four waves through LDS, then - plain stores, no atomics - over the
 // workgroups by a second launch.
@@ -14,7 +16,6 @@
 
 namespace {
 
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float add_halves(float a, float b) {         // lanes 0-31: a summed over the halves; lanes 32-63: b
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
