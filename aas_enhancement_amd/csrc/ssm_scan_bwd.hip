@@ -8,7 +8,8 @@
 // the run, holding a and p of its frames in registers, then back through them.  (States kept every 16 frames and the exponentials
 // formed twice was 289 us where this was 275, at 4096 x 4 x 1024 in bf16; now 263, at 200 x 30 x 1000 in fp32 91.  All 16 frames' a and p
 // do not fit the registers.)  Bound by instruction issue (105 a frame and wave, VALU active in 77 % of the busy cycles) at two waves a
-// SIMD; held to three by launch bounds it spills: 561 us.  dB and dC are sums over channels: eight values a lane (four
+// SIMD; held to three by launch bounds it spills: 561 us, and with a thread's own elements parked in LDS, where it nearly fits, three waves
+// were no faster (pass 578 us against 507).  dB and dC are sums over channels: eight values a lane (four
 // states x {dB, dC}) over the 16 channels of a wave go by exchanges that halve the number of values with the number of lanes still to
 // add (lane halves, rows of 16, then within the row), then over the four waves through LDS, then - plain stores, no atomics - over the
 // workgroups by a second launch.
