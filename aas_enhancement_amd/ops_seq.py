@@ -17,7 +17,6 @@ from ._lib import check, lib, ptr, require_cuda
 
 _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # include/aas_hip.h: AAS_DT_*
 
-
 _raw_stream = torch._C._cuda_getCurrentRawStream     # what torch.cuda.current_stream().cuda_stream ends in, without the object (3-6 us a call)
 _empty = torch.empty
 
@@ -90,7 +89,7 @@ def _activation(who, name, t, like=None, shape=None):
         _bad(who, "%s is %s on %s, expected %s on %s" % (name, t.dtype, t.device, like.dtype, like.device))
     if shape is not None and tuple(t.shape) != tuple(shape):
         _bad(who, "%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if t.dim() == 0 or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def _param(who, name, t, like, shape):
@@ -244,14 +243,14 @@ class _SsmScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, dt, A, B, C, D, z, dt_bias, softplus, lengths):
         y, hsave = _scan_fwd(x, dt, A, B, C, D, z, dt_bias, softplus, lengths, None, True)
-        ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, lengths)
-        ctx.hsave, ctx.softplus = hsave, softplus
+        ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, lengths, hsave)
+        ctx.softplus = softplus
         return y
 
     @staticmethod
     @_first_order
     def backward(ctx, dy):
-        x, dt, A, B, C, D, z, dt_bias, lengths = ctx.saved_tensors
+        x, dt, A, B, C, D, z, dt_bias, lengths, hsave = ctx.saved_tensors
         T, N, Ch = x.shape
         S, G = A.shape[1], B.shape[2]
         if dy.stride(-1) != 1:
@@ -263,7 +262,7 @@ class _SsmScan(torch.autograd.Function):
         dbias = None if dt_bias is None else A.new_empty((Ch,))
         ws = _ws(lib().aas_ssm_scan_bwd_ws_bytes(T, N, Ch, S, G), x.device)
         d = _scan_desc(x, dt, A, B, C, D, z, dt_bias, ctx.softplus, lengths)
-        check(lib().aas_ssm_scan_bwd(_stream(x), d, dy.data_ptr(), dy.stride(0), dy.stride(1), ctx.hsave.data_ptr(), dx.data_ptr(),
+        check(lib().aas_ssm_scan_bwd(_stream(x), d, dy.data_ptr(), dy.stride(0), dy.stride(1), hsave.data_ptr(), dx.data_ptr(),
                                      ddt.data_ptr(), ptr(dz), dB.data_ptr(), dC.data_ptr(), dA.data_ptr(), ptr(dD), ptr(dbias), ptr(ws)),
               "aas_ssm_scan_bwd")
         return dx, ddt, dA, dB, dC, dD, dz, dbias, None, None
@@ -350,13 +349,15 @@ def _dropout_call(x, drop, seed_dev, used):
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, drop):
-        ctx.drop = drop
+        ctx.drop = drop[:3]
+        ctx.save_for_backward(drop[4])
         return _dropout_call(x, drop, drop[3], drop[4])
 
     @staticmethod
     @_first_order
     def backward(ctx, dy):
-        return _dropout_call(dy.contiguous(), ctx.drop, ctx.drop[4], None), None
+        used, = ctx.saved_tensors
+        return _dropout_call(dy.contiguous(), ctx.drop, used, None), None
 
 
 @_on_device
@@ -388,7 +389,7 @@ def _res_fwd(x, x_ld, residual, res_ld, weight, bias, scale, eps, layer, drop, w
 
 
 def _res_bwd(ctx, dy, dr):
-    kept, x, weight, bias, scale = ctx.saved_tensors
+    kept, x, weight, bias, scale, stat, used = ctx.saved_tensors
     need, drop = ctx.needs_input_grad, ctx.drop
     C = kept.shape[-1]
     R = kept.numel() // C
@@ -405,8 +406,8 @@ def _res_bwd(ctx, dy, dr):
     dw, db, ds = (_empty(C, device=dev, dtype=torch.float32) if n else None for n in need[2:5])
     ws = _ws(lib().aas_residual_norm_bwd_ws_bytes(R, C), dev) if need[2] or need[3] or need[4] else None
     check(lib().aas_residual_norm_bwd(_stream(kept), _DT[ctx.x_dtype], _DT[kept.dtype], R, C, ptr(args[0]), args[1], ptr(args[2]), args[3], kept.data_ptr(),
-                                      ctx.kept_ld, ptr(x), ctx.x_ld, ctx.stat.data_ptr(), ptr(weight), ptr(scale), ctx.layer, drop[0], drop[1],
-                                      drop[2], ptr(drop[4]), ptr(dx), ptr(dres), ptr(dw), ptr(db), ptr(ds), ptr(ws)), "aas_residual_norm_bwd")
+                                      ctx.kept_ld, ptr(x), ctx.x_ld, stat.data_ptr(), ptr(weight), ptr(scale), ctx.layer, drop[0], drop[1],
+                                      drop[2], ptr(used), ptr(dx), ptr(dres), ptr(dw), ptr(db), ptr(ds), ptr(ws)), "aas_residual_norm_bwd")
     return dx, dres, dw, db, ds, None, None, None
 
 
@@ -417,9 +418,9 @@ class _ResidualNorm(torch.autograd.Function):
     def forward(ctx, x, residual, weight, bias, scale, eps, layer, drop):
         x, x_ld = _rows(x)
         res, res_ld = (None, 0) if residual is None else _rows(residual)
-        y, r, ctx.stat = _res_fwd(x, x_ld, res, res_ld, weight, bias, scale, eps, layer, drop, True, True)
-        ctx.save_for_backward(r, x if ctx.needs_input_grad[4] else None, weight, bias, scale)
-        ctx.x_dtype, ctx.x_ld, ctx.kept_ld, ctx.layer, ctx.drop = x.dtype, x_ld, x.shape[-1], layer, drop
+        y, r, stat = _res_fwd(x, x_ld, res, res_ld, weight, bias, scale, eps, layer, drop, True, True)
+        ctx.save_for_backward(r, x if ctx.needs_input_grad[4] else None, weight, bias, scale, stat, drop[4])
+        ctx.x_dtype, ctx.x_ld, ctx.kept_ld, ctx.layer, ctx.drop = x.dtype, x_ld, x.shape[-1], layer, drop[:3]
         ctx.set_materialize_grads(False)
         return y, r
 
@@ -438,9 +439,9 @@ class _Norm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, scale, eps, layer, drop):
         xr, x_ld = _rows(x)
-        y, _, ctx.stat = _res_fwd(xr, x_ld, None, 0, weight, bias, None, eps, layer, drop, False, True)
-        ctx.save_for_backward(xr, None, weight, bias, None)
-        ctx.x_dtype, ctx.x_ld, ctx.kept_ld, ctx.layer, ctx.drop = x.dtype, x_ld, x_ld, layer, drop
+        y, _, stat = _res_fwd(xr, x_ld, None, 0, weight, bias, None, eps, layer, drop, False, True)
+        ctx.save_for_backward(xr, None, weight, bias, None, stat, None)
+        ctx.x_dtype, ctx.x_ld, ctx.kept_ld, ctx.layer, ctx.drop = x.dtype, x_ld, x_ld, layer, drop[:3]
         ctx.set_materialize_grads(False)
         return y, x
 

@@ -555,6 +555,22 @@ def test_block_streams_frame_by_frame(ops):
     assert float((cs - c1).abs().max()) <= 2e-6 * float(cs.abs().max()) and float((ss - s1).abs().max()) <= 2e-6 * float(ss.abs().max())
 
 
+def test_backward_frees_what_forward_kept(ops):
+    """A loss that lives on after its backward pass (for a log line) holds none of the states kept for it."""
+    T, N, Ch, S = 256, 2, 256, 64
+    x, A = torch.randn(T, N, Ch, device="cuda", requires_grad=True), -torch.ones(Ch, S, device="cuda")
+    B = torch.randn(T, N, S, device="cuda")
+    kept = T // 8 * N * Ch * S * 4
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    loss = ops.ssm_scan(x, x, A, B, B).sum()
+    assert torch.cuda.memory_allocated() - before >= kept
+    loss.backward()
+    assert torch.cuda.memory_allocated() - before < kept // 2                  # x.grad, and the loss
+    scalar = torch.tensor(2.0, device="cuda")
+    assert float(ops.dropout(scalar, 0.5, 1)) in (0.0, 4.0)                    # no dimensions
+
+
 def test_first_derivatives_only(ops):
     """A recorded backward pass is fine as long as nobody differentiates through it."""
     x = torch.randn(4, 2, 8, device="cuda", requires_grad=True)
