@@ -234,7 +234,8 @@ bool conv_args_ok(const char* who, int dtype, int T, int N, int C, int K) {
     if (!aas_dt_ok(dtype)) { aas_set_error("%s: dtype %d", who, dtype); return false; }
     if (T < 0 || N < 0 || C < 0 || T > (1 << 30)) { aas_set_error("%s: T = %d, N = %d, C = %d", who, T, N, C); return false; }
     if (K < 2 || K > 4) { aas_set_error("%s: K = %d, must be 2, 3 or 4", who, K); return false; }
-    if (C > (1 << 24) || (int64_t)N * C > ((int64_t)1 << 36)) { aas_set_error("%s: N = %d, C = %d too large", who, N, C); return false; }
+    // (a launch has fewer than 2^32 threads)
+    if (C > (1 << 24) || (int64_t)N * cdiv(C, 4) > ((int64_t)1 << 30)) { aas_set_error("%s: N = %d, C = %d too large", who, N, C); return false; }
     return true;
 }
 

@@ -344,7 +344,6 @@ extern "C" int aas_ssm_scan_bwd(aasStream_t stream, const aasScan* d, const void
     const bool empty = d->T == 0 || d->N == 0;
     if (d->Ch == 0) return 0;
     AAS_CHECK(dA != nullptr, "%s: null pointer", who);
-    AAS_CHECK((int64_t)d->Ch * (d->S + 2) <= 0x7fffffff, "%s: Ch = %d too large", who, d->Ch);
     if (!empty) {
         const BwdWs w = bwd_ws(d->T, d->N, d->Ch, d->S, d->G);
         const ScanChunks ck = bwd_chunks(d->T, d->N, d->Ch, d->G);

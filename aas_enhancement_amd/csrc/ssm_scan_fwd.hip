@@ -214,7 +214,8 @@ int scan_check(const char* who, const aasScan* d) {
     AAS_CHECK(d->T <= 0x7fffffff - 2 * SCAN_TT, "%s: T = %d too long", who, d->T);
     AAS_CHECK(d->S >= 1 && d->S <= 64, "%s: S = %d, must be 1 to 64", who, d->S);
     AAS_CHECK(d->G >= 1 && d->Ch % d->G == 0, "%s: Ch = %d is no multiple of G = %d", who, d->Ch, d->G);
-    AAS_CHECK((int64_t)d->N * (cdiv(d->Ch / d->G, SCAN_CH) * (int64_t)d->G) <= 0x7fffffff, "%s: N = %d, Ch = %d too large", who, d->N, d->Ch);
+    // (a launch has fewer than 2^32 threads, 256 a workgroup; the finishing one a workgroup per 16 of Ch (S + 2) sums)
+    AAS_CHECK((int64_t)d->N * (cdiv(d->Ch / d->G, SCAN_CH) * (int64_t)d->G) <= (1 << 23) && (int64_t)d->Ch * (d->S + 2) <= (1 << 27), "%s: N = %d, Ch = %d too large", who, d->N, d->Ch);
     if (d->T == 0 || d->N == 0 || d->Ch == 0) return 0;
     AAS_CHECK(d->x && d->dt && d->A && d->B && d->C, "%s: null pointer", who);
     return 0;

@@ -159,7 +159,10 @@ def test_c_entry_points_refuse_without_a_gpu():
     bad(L.aas_causal_conv1d_fwd(None, 0, 1, 1, 1, 4, None, 1, 1, one, None, 1, None, None, one), b"null")
     bad(L.aas_causal_conv1d_bwd(None, 0, -1, 1, 1, 4, one, 1, 1, one, None, 1, None, one, 1, 1, one, one, one, one), b"T = -1")
     bad(L.aas_causal_conv1d_bwd(None, 0, 1, 1, 1, 4, one, 1, 1, one, None, 1, None, one, 1, 1, one, one, one, None), b"null")
-    desc = lambda S=16, G=1, size=ops_seq._SCAN.size: ops_seq._SCAN.pack(size, 0, 1, 1, 4, S, G, 1, *[0] * 21)   # noqa: E731
+    bad(L.aas_causal_conv1d_fwd(None, 0, 1, 1 << 30, 8, 4, one, 1, 1, one, None, 1, None, None, one), b"too large")
+    desc = lambda S=16, G=1, size=ops_seq._SCAN.size, N=1, Ch=4: ops_seq._SCAN.pack(size, 0, 1, N, Ch, S, G, 1, *[0] * 21)   # noqa: E731
+    bad(L.aas_ssm_scan_fwd(None, desc(N=(1 << 23) + 1), None, one, None, None), b"too large")
+    bad(L.aas_ssm_scan_fwd(None, desc(S=64, Ch=1 << 22), None, one, None, None), b"too large")
     bad(L.aas_ssm_scan_fwd(None, desc(), None, one, None, None), b"null")
     bad(L.aas_ssm_scan_fwd(None, desc(S=65), None, one, None, None), b"S = 65")
     bad(L.aas_ssm_scan_bwd(None, desc(G=3), one, 1, 1, one, one, one, None, one, one, one, None, None, one), b"no multiple")
