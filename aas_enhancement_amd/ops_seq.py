@@ -136,8 +136,21 @@ def _wants_grad(*ts):
     return False
 
 
+# The backward passes ask for the layouts of what they read again: what a saved-tensor hook hands back
+# (torch.autograd.graph.save_on_cpu) holds the values that were saved, not their strides.
+def _unit(t):
+    """An activation with its channels side by side."""
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _whole(*ts):
+    """Parameters, statistics and states, contiguous."""
+    return [t if t is None or t.is_contiguous() else t.contiguous() for t in ts]
+
+
 def _rows(t):
     """-> (tensor, row pitch): the leading dimensions as uniformly spaced rows, copied where they are not."""
+    t = _unit(t)
     if t.is_contiguous():
         return t, t.shape[-1]
     pitch, seen = None, 1
@@ -173,10 +186,10 @@ class _CausalConv1d(torch.autograd.Function):
     @_first_order
     def backward(ctx, dy):
         x, weight, bias, lengths = ctx.saved_tensors
+        x, dy = _unit(x), _unit(dy)
+        weight, bias, lengths = _whole(weight, bias, lengths)
         T, N, C = x.shape
         K = weight.shape[1]
-        if dy.stride(-1) != 1:
-            dy = dy.contiguous()
         need = ctx.needs_input_grad
         dx = _empty((T, N, C), device=x.device, dtype=x.dtype) if need[0] else None
         dw = torch.empty_like(weight) if need[1] else None
@@ -251,10 +264,10 @@ class _SsmScan(torch.autograd.Function):
     @_first_order
     def backward(ctx, dy):
         x, dt, A, B, C, D, z, dt_bias, lengths, hsave = ctx.saved_tensors
+        x, dt, B, C, z, dy = map(_unit, (x, dt, B, C, z, dy))
+        A, D, dt_bias, lengths, hsave = _whole(A, D, dt_bias, lengths, hsave)
         T, N, Ch = x.shape
         S, G = A.shape[1], B.shape[2]
-        if dy.stride(-1) != 1:
-            dy = dy.contiguous()
         dx, ddt = x.new_empty((T, N, Ch)), x.new_empty((T, N, Ch))
         dz = None if z is None else x.new_empty((T, N, Ch))
         dB, dC, dA = x.new_empty((T, N, G, S)), x.new_empty((T, N, G, S)), A.new_empty((Ch, S))
@@ -356,7 +369,7 @@ class _Dropout(torch.autograd.Function):
     @staticmethod
     @_first_order
     def backward(ctx, dy):
-        used, = ctx.saved_tensors
+        used, = _whole(*ctx.saved_tensors)
         return _dropout_call(dy.contiguous(), ctx.drop, used, None), None
 
 
@@ -389,7 +402,10 @@ def _res_fwd(x, x_ld, residual, res_ld, weight, bias, scale, eps, layer, drop, w
 
 
 def _res_bwd(ctx, dy, dr):
-    kept, x, weight, bias, scale, stat, used = ctx.saved_tensors
+    kept, x, weight, scale, stat, used = ctx.saved_tensors
+    kept, kept_ld = _rows(kept)
+    x, x_ld = (None, 0) if x is None else _rows(x)
+    weight, scale, stat, used = _whole(weight, scale, stat, used)
     need, drop = ctx.needs_input_grad, ctx.drop
     C = kept.shape[-1]
     R = kept.numel() // C
@@ -399,14 +415,13 @@ def _res_bwd(ctx, dy, dr):
         if g is None:
             args += [None, 0]
         else:
-            g, ld = _rows(g if g.stride(-1) == 1 or C == 1 else g.contiguous())
-            args += [g, ld]
+            args += _rows(g)
     dx = _empty(shape, device=dev, dtype=ctx.x_dtype) if need[0] else None
     dres = _empty(shape, device=dev, dtype=kept.dtype) if need[1] else None
     dw, db, ds = (_empty(C, device=dev, dtype=torch.float32) if n else None for n in need[2:5])
     ws = _ws(lib().aas_residual_norm_bwd_ws_bytes(R, C), dev) if need[2] or need[3] or need[4] else None
     check(lib().aas_residual_norm_bwd(_stream(kept), _DT[ctx.x_dtype], _DT[kept.dtype], R, C, ptr(args[0]), args[1], ptr(args[2]), args[3], kept.data_ptr(),
-                                      ctx.kept_ld, ptr(x), ctx.x_ld, stat.data_ptr(), ptr(weight), ptr(scale), ctx.layer, drop[0], drop[1],
+                                      kept_ld, ptr(x), x_ld, stat.data_ptr(), ptr(weight), ptr(scale), ctx.layer, drop[0], drop[1],
                                       drop[2], ptr(used), ptr(dx), ptr(dres), ptr(dw), ptr(db), ptr(ds), ptr(ws)), "aas_residual_norm_bwd")
     return dx, dres, dw, db, ds, None, None, None
 
@@ -419,8 +434,8 @@ class _ResidualNorm(torch.autograd.Function):
         x, x_ld = _rows(x)
         res, res_ld = (None, 0) if residual is None else _rows(residual)
         y, r, stat = _res_fwd(x, x_ld, res, res_ld, weight, bias, scale, eps, layer, drop, True, True)
-        ctx.save_for_backward(r, x if ctx.needs_input_grad[4] else None, weight, bias, scale, stat, drop[4])
-        ctx.x_dtype, ctx.x_ld, ctx.kept_ld, ctx.layer, ctx.drop = x.dtype, x_ld, x.shape[-1], layer, drop[:3]
+        ctx.save_for_backward(r, x if ctx.needs_input_grad[4] else None, weight, scale, stat, drop[4])
+        ctx.x_dtype, ctx.layer, ctx.drop = x.dtype, layer, drop[:3]
         ctx.set_materialize_grads(False)
         return y, r
 
@@ -440,8 +455,8 @@ class _Norm(torch.autograd.Function):
     def forward(ctx, x, residual, weight, bias, scale, eps, layer, drop):
         xr, x_ld = _rows(x)
         y, _, stat = _res_fwd(xr, x_ld, None, 0, weight, bias, None, eps, layer, drop, False, True)
-        ctx.save_for_backward(xr, None, weight, bias, None, stat, None)
-        ctx.x_dtype, ctx.x_ld, ctx.kept_ld, ctx.layer, ctx.drop = x.dtype, x_ld, x_ld, layer, drop[:3]
+        ctx.save_for_backward(xr, None, weight, None, stat, None)
+        ctx.x_dtype, ctx.layer, ctx.drop = x.dtype, layer, drop[:3]
         ctx.set_materialize_grads(False)
         return y, x
 
@@ -495,17 +510,17 @@ class _GatedNorm(torch.autograd.Function):
     def forward(ctx, x, gate, weight, eps, groups, norm_first):
         (x, x_ld), (gate, gate_ld) = _rows(x), _rows(gate)
         ctx.save_for_backward(x, gate, weight)
-        ctx.args = (x_ld, gate_ld, eps, groups, norm_first)
+        ctx.args = (eps, groups, norm_first)
         return _gated_fwd(x, x_ld, gate, gate_ld, weight, eps, groups, norm_first)
 
     @staticmethod
     @_first_order
     def backward(ctx, dy):
         x, gate, weight = ctx.saved_tensors
-        x_ld, gate_ld, eps, groups, norm_first = ctx.args
+        eps, groups, norm_first = ctx.args
+        (x, x_ld), (gate, gate_ld), (dy, dy_ld), (weight,) = _rows(x), _rows(gate), _rows(dy), _whole(weight)
         C = x.shape[-1]
         R = x.numel() // C
-        dy, dy_ld = _rows(dy if dy.stride(-1) == 1 or C == 1 else dy.contiguous())
         need = ctx.needs_input_grad
         dx, dg = (_empty(x.shape, device=x.device, dtype=x.dtype) if n else None for n in need[:2])
         dw = torch.empty_like(weight) if need[2] else None

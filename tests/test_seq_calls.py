@@ -1,0 +1,104 @@
+"""CPU (-m "not gpu"): calls of the causal sequence operators that their documentation allows, up to the library's door: host tensors pass
+for device tensors and every entry point is replaced by one that writes its arguments down."""
+import pytest
+import torch
+
+from aas_enhancement_amd import _lib, ops_seq
+
+
+class Recorder:
+    """In place of the library: entry points by name, each call's arguments kept."""
+
+    def __init__(self):
+        self.calls, self.barred = [], {}
+
+    def __getattr__(self, name):
+        def entry(*args):
+            assert len(args) == len(_lib.SIGNATURES[name]), name
+            if name.endswith("_ws_bytes"):
+                return 64
+            self.calls.append((name, args))
+            given = [v for a in args for v in (ops_seq._SCAN.unpack(a) if isinstance(a, bytes) else (a,))]
+            assert not set(given) & set(self.barred), name        # (while they live: an address may be another's afterwards)
+            return 0
+        return entry
+
+    def args(self, name):
+        return [a for n, a in self.calls if n == name][-1]
+
+
+@pytest.fixture
+def door(monkeypatch):
+    rec = Recorder()
+    monkeypatch.setattr(ops_seq, "require_cuda", lambda *t: None)
+    monkeypatch.setattr(ops_seq, "_stream", lambda t: 0)
+    monkeypatch.setattr(ops_seq, "lib", lambda: rec)
+    return rec
+
+
+class relaid:
+    """Saved tensors come back contiguous, as from torch.autograd.graph.save_on_cpu; `strides` knows what lies at an address."""
+
+    def __init__(self, order=lambda t: t.contiguous()):
+        self.strides, self.kept, self.order = {}, [], order
+
+    def __enter__(self):
+        self.hooks = torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(memory_format=torch.contiguous_format), self.unpack)
+        self.hooks.__enter__()
+        return self
+
+    def __exit__(self, *e):
+        self.hooks.__exit__(*e)
+
+    def unpack(self, t):
+        t = self.order(t)
+        self.kept.append(t)
+        self.strides[t.data_ptr()] = t.stride()
+        return t
+
+
+def test_gated_norm_reads_saved_rows_where_they_lie(door):
+    x, wide = torch.randn(6, 16), torch.randn(6, 24, requires_grad=True)
+    w = torch.ones(8, requires_grad=True)
+    with relaid() as s:
+        ops_seq.gated_norm(x[:, :8], wide[:, 4:12], w).sum().backward()
+    a = door.args("aas_gated_norm_bwd")
+    assert s.strides[a[7]] == (8, 1) and a[8] == 8
+    assert s.strides[a[9]] == (8, 1) and a[10] == 8
+
+
+@pytest.mark.parametrize("full", [False, True], ids=["norm", "residual"])
+def test_residual_norm_reads_saved_rows_where_they_lie(door, full):
+    wide, w = torch.randn(6, 24), torch.ones(8, requires_grad=True)
+    res, scale = (torch.randn(6, 8), torch.ones(8, requires_grad=True)) if full else (None, None)
+    with relaid() as s:
+        ops_seq.residual_norm(wide[:, 4:12], res, w, scale=scale)[0].sum().backward()
+    a = door.args("aas_residual_norm_bwd")
+    assert s.strides[a[9]] == (8, 1) and a[10] == 8
+    if full:
+        assert s.strides[a[11]] == (8, 1) and a[12] == 8
+
+
+def test_saved_tensors_that_come_back_spaced_out(door):
+    """A hook may also hand everything back at other strides: all is read as it lies, or copied first."""
+    apart = relaid(lambda t: torch.stack([t, t], -1)[..., 0])
+    door.barred = apart.strides
+    x, w = torch.randn(4, 3, 8), torch.randn(8, 4, requires_grad=True)
+    A, B, D = torch.randn(8, 16, requires_grad=True), torch.randn(4, 3, 16), torch.ones(8)
+    n = torch.full((3,), 4, dtype=torch.int32)
+    g, r, v, seed = torch.ones(4, 3, 8), torch.randn(6, 8), torch.ones(8, requires_grad=True), torch.zeros(2, dtype=torch.int64)
+    with apart:
+        ops_seq.causal_conv1d(x, w, D, lengths=n).backward(g)
+        a = door.args("aas_causal_conv1d_bwd")
+        assert a[7:9] == (24, 8) and a[14:16] == (24, 8)
+        ops_seq.ssm_scan(x, x, A, B, B, D=D, z=x, dt_bias=D, lengths=n).backward(g)
+        f = ops_seq._SCAN.unpack(door.args("aas_ssm_scan_bwd")[1])
+        assert f[17:23] == (24, 8) * 3 and f[23:] == (48, 16, 16) * 2
+        ops_seq.gated_norm(r, r, v).backward(torch.ones(6, 8))
+        a = door.args("aas_gated_norm_bwd")
+        assert a[6] == a[8] == a[10] == 8
+        ops_seq.residual_norm(r, r, v, D, scale=v, p=0.5, seed=seed)[0].backward(torch.ones(6, 8))
+        a = door.args("aas_residual_norm_bwd")
+        assert a[6] == a[10] == a[12] == 8
+        ops_seq.dropout(r.requires_grad_(), 0.5, seed).backward(torch.ones(6, 8))
+    assert apart.strides
