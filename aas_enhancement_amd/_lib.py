@@ -184,3 +184,12 @@ def require_cuda(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise RuntimeError("aas_enhancement_amd ops run on the MI355X only: got a %s tensor (no CPU fallback)" % t.device)
+
+
+def require_f32(*tensors):
+    """For the operators that read and write fp32 only: a 16-bit tensor's pointer would be read over twice its bytes."""
+    require_cuda(*tensors)
+    for t in tensors:
+        if t is not None and t.dtype is not torch.float32:
+            raise RuntimeError("aas_enhancement_amd: got a %s tensor where the operator computes in fp32 (16-bit activations are for the causal sequence "
+                               "operators alone)" % t.dtype)

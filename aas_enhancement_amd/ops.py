@@ -9,7 +9,7 @@ channels-last [N,T,C]; the module boundary keeps the reference's [N,C,T].
 import torch
 
 from . import knobs
-from ._lib import check, lib, ptr, require_cuda, stream
+from ._lib import check, lib, ptr, require_f32, stream
 
 NT, NN, TN = 0, 1, 2
 
@@ -932,7 +932,7 @@ class _Layout(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, kind):
-        require_cuda(x)
+        require_f32(x)
         ctx.kind = kind
         return _Layout.FWD[kind](_c(x))
 
@@ -954,7 +954,7 @@ class _LayoutCatNCT(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, a, b):
-        require_cuda(a, b)
+        require_f32(a, b)
         a, b = _c(a), _c(b)
         Na, C, Ta = a.shape
         Nb, Tb = b.shape[0], b.shape[2]
@@ -990,7 +990,7 @@ class _LayoutPairedCat(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, leaf, mixture, cleans):
-        require_cuda(leaf, mixture, cleans)
+        require_f32(leaf, mixture, cleans)
         leaf, mixture, cleans = _c(leaf), _c(mixture), _c(cleans)
         N, F, T = leaf.shape
         assert tuple(mixture.shape) == (N, F, T) and tuple(cleans.shape) == (N, F, T)
@@ -1022,7 +1022,7 @@ class _LinearRows(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, W, b, rs=None):
-        require_cuda(x, W)
+        require_f32(x, W, b)
         x = _c(x)
         W2 = _c(W).view(W.shape[0], -1)
         x2 = x.view(-1, x.shape[-1])
@@ -1698,7 +1698,7 @@ class _BiRNNLayer(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w_ih, w_hh, w_ih_r, w_hh_r, kind, residual, rs=None, lid=0):
-        require_cuda(x, w_ih, w_hh)
+        require_f32(x, w_ih, w_hh, w_ih_r, w_hh_r)
         rs = RowWeights.of(rs)
         ctx.rs, ctx.lid = rs, lid
         ctx.params = (w_ih, w_hh, w_ih_r, w_hh_r)  # the nn.Parameters themselves (for the direct-accumulate path)
@@ -1760,7 +1760,7 @@ class _BatchNormRows(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, gamma, beta, running_mean, running_var, eps, momentum, slope, nbt=None):
-        require_cuda(x, gamma)
+        require_f32(x, gamma, beta, running_mean, running_var)
         x = _c(x)
         C = x.shape[-1]
         R = x.numel() // C
@@ -1820,7 +1820,7 @@ class _LeakyReLU(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, slope):
-        require_cuda(x)
+        require_f32(x)
         x = _c(x)
         y = torch.empty_like(x)
         check(lib().aas_leaky_relu_f32(stream(), ptr(y), ptr(x), ptr(x), float(slope), x.numel()), "aas_leaky_relu_f32")
@@ -1843,7 +1843,7 @@ def leaky_relu(x, slope):
 
 def batchnorm_eval(x, gamma, beta, running_mean, running_var, eps=1e-5, slope=1.0):
     """Eval-mode BatchNorm (running statistics) + fused LeakyReLU; inference only (no autograd)."""
-    require_cuda(x, gamma)
+    require_f32(x, gamma, beta, running_mean, running_var)
     x = _c(x.detach())
     C = x.shape[-1]
     y = torch.empty_like(x)
@@ -1854,7 +1854,7 @@ def batchnorm_eval(x, gamma, beta, running_mean, running_var, eps=1e-5, slope=1.
 
 def softmax_rows(x):
     """softmax over the last dim (C <= 64); inference only (InferenceBatchSoftmax in eval mode, model.py:58-64)."""
-    require_cuda(x)
+    require_f32(x)
     x = _c(x.detach())
     C = x.shape[-1]
     y = torch.empty_like(x)
@@ -1889,7 +1889,7 @@ class _Conv1dCL(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, W, b, stride):
-        require_cuda(x, W)
+        require_f32(x, W, b)
         x = _c(x)
         N, T, F = x.shape
         M, _, KW = W.shape
@@ -1945,7 +1945,7 @@ class _L1Sum(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, a, b):
-        require_cuda(a, b)
+        require_f32(a, b)
         a, b = _c(a), _c(b)
         acc = torch.zeros((1,), device=a.device, dtype=torch.float64)
         check(lib().aas_l1_fwd(stream(), ptr(a), ptr(b), a.numel(), ptr(acc)), "aas_l1_fwd")
@@ -1995,7 +1995,7 @@ class _L1Pair(torch.autograd.Function):
         """target_grad (a list, optional): the gradient wrt `leaf` AS THE TARGET of the first loss is appended to it instead of
         being returned to autograd - the caller adds it where it sums the gradients arriving at `enhanced` anyway (one three-input
         add3 launch instead of an autograd accumulation launch plus a two-input add3)."""
-        require_cuda(ae, leaf, clean)
+        require_f32(ae, leaf, clean)
         ctx.target_grad = target_grad
         ae, leaf, clean = _c(ae), _c(leaf), _c(clean)
         assert acc.dtype == torch.float64 and acc.numel() == 2
@@ -2063,7 +2063,7 @@ class _L1Scaled(torch.autograd.Function):
     def forward(ctx, a, b, scale, acc, grad_out=None):
         """grad_out (a list, optional): the gradient wrt `a` is appended to it instead of being returned to autograd - the caller
         adds it where it sums the gradients arriving at that tensor anyway (no autograd accumulation launch)."""
-        require_cuda(a, b)
+        require_f32(a, b)
         a, b = _c(a), _c(b)
         assert acc.dtype == torch.float64 and acc.numel() >= 1
         check(lib().aas_l1_fwd(stream(), ptr(a), ptr(b), a.numel(), ptr(acc)), "aas_l1_fwd")
@@ -2133,7 +2133,7 @@ class _CTC(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, acts, labels, act_lens, label_lens, blank, prepared):
-        require_cuda(acts)
+        require_f32(acts)
         acts = _c(acts)
         T, N, C = acts.shape
         dev = acts.device
@@ -2177,7 +2177,7 @@ class _CTCScaled(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, acts, blank, prepared, scale):
-        require_cuda(acts)
+        require_f32(acts)
         acts = _c(acts)
         T, N, C = acts.shape
         dev = acts.device
