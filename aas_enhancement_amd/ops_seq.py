@@ -12,6 +12,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad as _fw
 
 from ._lib import check, lib, ptr, require_cuda
 
@@ -58,6 +59,8 @@ def _first_order(backward):
     refuse to be differentiated wherever they depend on something that wants a gradient."""
     @functools.wraps(backward)
     def wrapped(ctx, *g):
+        if _fw._current_level >= 0:
+            _no_tangents(*g, *ctx.saved_tensors)
         if not torch.is_grad_enabled():
             return backward(ctx, *g)
         with torch.no_grad():
@@ -128,7 +131,16 @@ def _written(state):
         torch.autograd.graph.increment_version(state)
 
 
+def _no_tangents(*ts):
+    """Inside a torch.autograd.forward_ad level: the kernels would hand the values on and drop the tangents."""
+    for t in ts:
+        if isinstance(t, torch.Tensor) and _fw.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("the causal sequence operators have no forward-mode derivatives")
+
+
 def _wants_grad(*ts):
+    if _fw._current_level >= 0:
+        _no_tangents(*ts)
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:

@@ -126,3 +126,39 @@ def test_fp32_layers_refuse_other_types(monkeypatch, dtype):
     for call in calls:
         with pytest.raises(RuntimeError, match="computes in fp32"):
             call()
+
+
+def _forms(x, w, A, B, v):
+    """Every operator on the given tensors: activations [4, 2, 8], weight [8, 4], A [8, 16], B [4, 2, 16], channel vector [8]."""
+    state = lambda *s: torch.zeros(*s)     # noqa: E731
+    return [lambda: ops_seq.causal_conv1d(x, w, v), lambda: ops_seq.causal_conv1d(x.detach(), w, v), lambda: ops_seq.causal_conv1d(x, w, v, state=state(2, 3, 8)),
+            lambda: ops_seq.ssm_scan(x, x, A, B, B, D=v, z=x, dt_bias=v), lambda: ops_seq.ssm_scan(x.detach(), x.detach(), A, B.detach(), B.detach()),
+            lambda: ops_seq.ssm_scan(x, x, A, B, B, state=state(2, 8, 16)), lambda: ops_seq.residual_norm(x), lambda: ops_seq.residual_norm(x.detach(), x, v),
+            lambda: ops_seq.residual_norm(x.detach(), x.detach(), scale=v), lambda: ops_seq.gated_norm(x, x, v), lambda: ops_seq.gated_norm(x.detach(), x),
+            lambda: ops_seq.dropout(x, 0.5, 1)]
+
+
+def test_forward_mode_derivatives_are_refused(door):
+    """A dual tensor's tangent is not dropped without a word - with gradients wanted, without, and in a backward pass."""
+    from torch.autograd import forward_ad as fw
+    shapes = [(4, 2, 8), (8, 4), (8, 16), (4, 2, 16), (8,)]
+    plain = [torch.randn(s) for s in shapes]
+    with fw.dual_level():
+        for f in _forms(*plain):
+            f()                                           # (no tangents: nothing to refuse)
+        dual = [fw.make_dual(t, torch.ones_like(t)) for t in plain]
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for f in _forms(*dual):
+                    with pytest.raises(NotImplementedError):
+                        f()
+        leaf = [t.clone().requires_grad_() for t in plain]
+        for f in _forms(*leaf):
+            try:
+                y = f()
+            except RuntimeError as e:                     # (states are for inference)
+                assert "inference" in str(e)
+                continue
+            y = y[0] if isinstance(y, tuple) else y
+            with pytest.raises(NotImplementedError):
+                torch.autograd.grad(y, [t for t in leaf if t.requires_grad], fw.make_dual(torch.ones_like(y), torch.ones_like(y)), allow_unused=True)
