@@ -183,6 +183,8 @@ extern "C" int aas_gated_norm_bwd(aasStream_t stream, int dtype, int64_t R, int 
                                   float* dweight, void* ws) {
     const char* who = "aas_gated_norm_bwd";
     if (!gated_args(who, dtype, R, C, groups)) return 1;
+    // (the launch that sums dweight has a workgroup of 256 per 16 columns, and fewer than 2^32 threads)
+    AAS_CHECK(!dweight || cdiv(C, 16) < (1 << 24), "%s: C = %d too large for a weight's gradient", who, C);
     hipStream_t s = (hipStream_t)stream;
     int P = 0;
     if (R > 0) {

@@ -162,3 +162,14 @@ def test_forward_mode_derivatives_are_refused(door):
             y = y[0] if isinstance(y, tuple) else y
             with pytest.raises(NotImplementedError):
                 torch.autograd.grad(y, [t for t in leaf if t.requires_grad], fw.make_dual(torch.ones_like(y), torch.ones_like(y)), allow_unused=True)
+
+
+def _refuses(rc, text):
+    assert rc == 1 and text in _lib.lib().aas_last_error(), (rc, _lib.lib().aas_last_error())
+
+
+def test_gated_norm_c_entry_refuses_a_gradient_launch_past_2_to_the_32():
+    """Before anything is launched (no rows: nothing would run but the sums of nothing)."""
+    one = 4096      # (never read)
+    L = _lib.lib()
+    _refuses(L.aas_gated_norm_bwd(None, 0, 0, 16384 * 16384, 16384, one, 8, one, 8, one, 8, None, 1e-5, 0, one, one, one, None), b"too large")
