@@ -146,7 +146,7 @@ bool gated_args(const char* who, int dtype, int64_t R, int C, int groups) {
     if (!aas_dt_ok(dtype)) { aas_set_error("%s: dtype %d", who, dtype); return false; }
     if (R < 0 || C < 1 || groups < 1 || C % groups) { aas_set_error("%s: R = %lld, C = %d, groups = %d", who, (long long)R, C, groups); return false; }
     if (C / groups > NORM_MAX_C) { aas_set_error("%s: %d channels a group, at most %d", who, C / groups, NORM_MAX_C); return false; }
-    if (groups > 65535 || R * groups > 0x7fffffff) { aas_set_error("%s: R = %lld, groups = %d too large", who, (long long)R, groups); return false; }
+    if (groups > 65535 || R > 0x7fffffff / groups) { aas_set_error("%s: R = %lld, groups = %d too large", who, (long long)R, groups); return false; }
     return true;
 }
 

@@ -173,3 +173,10 @@ def test_gated_norm_c_entry_refuses_a_gradient_launch_past_2_to_the_32():
     one = 4096      # (never read)
     L = _lib.lib()
     _refuses(L.aas_gated_norm_bwd(None, 0, 0, 16384 * 16384, 16384, one, 8, one, 8, one, 8, None, 1e-5, 0, one, one, one, None), b"too large")
+
+
+def test_gated_norm_c_entry_refuses_rows_times_groups_past_64_bits():
+    one = 4096      # (never read: pointers that are missing end the calls in any case)
+    L = _lib.lib()
+    _refuses(L.aas_gated_norm_fwd(None, 0, 1 << 62, 16, 4, None, 16, one, 16, None, 1e-5, 0, one), b"too large")
+    _refuses(L.aas_gated_norm_bwd(None, 0, 1 << 62, 16, 4, None, 16, one, 16, one, 16, None, 1e-5, 0, one, one, None, None), b"too large")
