@@ -31,6 +31,12 @@ def build(force=False, verbose=True):
     hdrs = [os.path.join(SRC, f) for f in os.listdir(SRC) if f.endswith(".h")]
     hdrs.append(os.path.join(os.path.dirname(HERE), "include", "aas_hip.h"))
     hdrs.append(os.path.join(os.path.dirname(HERE), "include", "aas_warpctc.h"))
+    # what the objects were compiled with lies beside them: another compiler or other flags compile everything again
+    command, record = " ".join([HIPCC] + FLAGS), os.path.join(OBJ, "command.txt")
+    if not os.path.exists(record) or open(record).read() != command:
+        force = True
+        if os.path.exists(record):
+            os.unlink(record)         # (a build that fails on the way leaves objects of both)
     jobs = []
     for f in srcs:
         src, obj = os.path.join(SRC, f), os.path.join(OBJ, f[:-4] + ".o")
@@ -49,6 +55,9 @@ def build(force=False, verbose=True):
             for s in ex.map(cc, jobs):
                 if verbose:
                     print("[build] compiled", os.path.basename(s), flush=True)
+    if jobs:
+        with open(record, "w") as f:
+            f.write(command)
     objs = [os.path.join(OBJ, f[:-4] + ".o") for f in srcs]
     if jobs or not os.path.exists(LIB):
         r = subprocess.run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs,
