@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(ScanDev a, const float*
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
         const int s0 = g * 16 + 4 * q;
-        A2[g] = on ? scan_states4(a.A + (int64_t)(b.c0 + cw) * a.S, s0, a.S, svec) * SCAN_LOG2E : zero;
+        A2[g] = on ? scan_rates4(a.A + (int64_t)(b.c0 + cw) * a.S, s0, a.S, svec) : zero;
         h[g] = on && !REV && state && k == 0 ? scan_states4(state + ch * a.S, s0, a.S, svec) : zero;
     }
     const f32x4 bias = a.dt_bias ? load4n<float, false>(a.dt_bias + b.c0 + lc, ln) : zero;

@@ -145,6 +145,18 @@ __device__ __forceinline__ void scan_put_states4(float* row, int s0, int S, bool
             if (s0 + j < S) row[s0 + j] = v[j];
 }
 
+// A log2(e) of the same states: exp(d A) is one exp2.  Brought inside the finite numbers (a NaN stays): a rate of -inf, or one that the
+// factor takes there, forgets everything in one frame, and d = 0 behind a row's end still leaves the state as it is (0 inf is none).
+__device__ __forceinline__ f32x4 scan_rates4(const float* row, int s0, int S, bool vec) {
+    f32x4 v = scan_states4(row, s0, S, vec) * SCAN_LOG2E;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        v[j] = v[j] < -3.4028234e38f ? -3.4028234e38f : v[j];
+        v[j] = v[j] > 3.4028234e38f ? 3.4028234e38f : v[j];
+    }
+    return v;
+}
+
 template <int NG, bool REV>
 __device__ __forceinline__ void scan_fold(f32x4 (&h)[NG], const f32x4 (&A2)[NG], const float* ends, const float* sums, int k, int nchunk, int64_t rows,
                                           int64_t ch, int S, int q, bool svec) {

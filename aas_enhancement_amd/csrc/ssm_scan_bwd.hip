@@ -66,7 +66,7 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
     f32x4 A2[NG], dA[NG], carry[NG];                                    // carry = a[t+1] g[t+1]
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-        A2[g] = on ? scan_states4(a.A + (int64_t)(b.c0 + cw) * a.S, g * 16 + 4 * q, a.S, svec) * SCAN_LOG2E : zero;
+        A2[g] = on ? scan_rates4(a.A + (int64_t)(b.c0 + cw) * a.S, g * 16 + 4 * q, a.S, svec) : zero;
         dA[g] = carry[g] = zero;
     }
     const int chunk = blockIdx.y;

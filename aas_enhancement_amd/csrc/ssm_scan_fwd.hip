@@ -23,14 +23,14 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanDev a, float* __restr
     const T* bp = (const T*)a.B + b.n * a.B_sn + b.grp * a.B_sg;
     const T* cp = (const T*)a.C + b.n * a.C_sn + b.grp * a.C_sg;
 
-    f32x4 A2[NG], h[NG];                                                // A log2(e): exp(d A) is one exp2
+    f32x4 A2[NG], h[NG];
     const int64_t srow = ((int64_t)b.n * a.Ch + b.c0 + cw) * a.S;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
         const int s0 = g * 16 + 4 * q;
         A2[g] = h[g] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (on) {
-            A2[g] = scan_states4(a.A + (int64_t)(b.c0 + cw) * a.S, s0, a.S, svec) * SCAN_LOG2E;
+            A2[g] = scan_rates4(a.A + (int64_t)(b.c0 + cw) * a.S, s0, a.S, svec);
             // (a split launch: the first chunk's end has the state in it; and the last chunk, which writes the new state, may finish first, so
             // the first one reads the copy that the carry launch left)
             if (state && a.nchunk == 1) h[g] = scan_states4(state + srow, s0, a.S, svec);
@@ -161,14 +161,14 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanDev a, int bvec, flo
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
         const int s0 = g * 16 + 4 * q;
-        const f32x4 A = scan_states4(a.A + (int64_t)c * a.S, s0, a.S, svec);
+        const f32x4 A2 = scan_rates4(a.A + (int64_t)c * a.S, s0, a.S, svec);
         f32x4 h = {0.f, 0.f, 0.f, 0.f};
         if (state) h = scan_states4(state + ch * a.S, s0, a.S, svec);
         const f32x4 B = bvec ? load4n<T, true>(bp + s0, a.S - s0) : load4n<T, false>(bp + s0, a.S - s0);
         const f32x4 C = bvec ? load4n<T, true>(cp + s0, a.S - s0) : load4n<T, false>(cp + s0, a.S - s0);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            h[j] = fmaf(__builtin_amdgcn_exp2f(d * (A[j] * SCAN_LOG2E)), h[j], dx * B[j]);
+            h[j] = fmaf(__builtin_amdgcn_exp2f(d * A2[j]), h[j], dx * B[j]);
             acc = fmaf(h[j], C[j], acc);
         }
         if (state) scan_put_states4(state + ch * a.S, s0, a.S, svec, h);

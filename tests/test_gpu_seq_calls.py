@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from tests.test_gpu_seq import ops, rnd  # noqa: F401
+from oracle import seq
+from tests.test_gpu_seq import close, dev, leaves, ops, rnd  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +32,29 @@ def test_saved_tensors_by_way_of_the_host(ops):
         away = grads()
     for a, b in zip(plain, away):
         assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------------------- scan: the ends of the ranges
+@pytest.mark.parametrize("rate", [float("-inf"), -3.2e38], ids=["infinite", "overflowing"])
+def test_scan_rates_without_memory(ops, rate):
+    """A = -inf (-exp of a large parameter): h = d x B of the frame alone, and what lies behind a row's end, inside its last tile too,
+    leaves the state as it is."""
+    T, N, Ch, S = 21, 3, 6, 5
+    g = torch.Generator().manual_seed(3)
+    x, dt, B, C, dy = rnd(g, T, N, Ch), rnd(g, T, N, Ch), rnd(g, T, N, S), rnd(g, T, N, S), rnd(g, T, N, Ch)
+    A = torch.full((Ch, S), rate)
+    n = torch.tensor([21, 2, 0], dtype=torch.int32)
+    for T1 in (T, 1):                                     # (one frame is a kernel of its own)
+        ref = seq.scan(x[:T1], dt[:T1], A, B[:T1], C[:T1], lengths=n, state=torch.ones(N, Ch, S))
+        mag = seq.scan(x[:T1], dt[:T1], A, B[:T1], C[:T1], lengths=n, state=torch.ones(N, Ch, S), mag=True)
+        state = torch.ones(N, Ch, S, device="cuda")
+        y = ops.ssm_scan(*map(dev, (x[:T1], dt[:T1], A, B[:T1], C[:T1])), lengths=dev(n), state=state)
+        close("y", y, ref["y"], mag["y"], S + 40)         # softplus, two products, a sum over the states
+        close("state", state, ref["state"], mag["state"], 40)
+    ins = leaves(x, dt, A, B, C)
+    ops.ssm_scan(*ins, lengths=dev(n)).backward(dev(dy))
+    finite = torch.full((Ch, S), -1e30)                   # the same decay, 0, and defined derivatives: q = g a h[t-1] is 0
+    ref, mag = (seq.scan(x, dt, finite, B, C, lengths=n, dy=dy, mag=m) for m in (False, True))
+    for name, t in zip(("dx", "ddt", "dB", "dC"), (ins[0], ins[1], ins[3], ins[4])):
+        close(name, t.grad, ref[name].view_as(t), mag[name].view_as(t), S + Ch + 60)
+    assert not ins[2].grad.any()
