@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
     }
     const int chunk = blockIdx.y;
     if (on && chunk + 1 < a.nchunk)
-        scan_fold<NG, true>(carry, A2, ends, sums, chunk * a.fine + a.fine - 1, a.nchunk * a.fine, (int64_t)a.N * a.Ch, (int64_t)b.n * a.Ch + b.c0 + cw, a.S, q, svec);
+        scan_fold<NG, true>(carry, A2, ends, sums, chunk * a.fine + a.fine - 1, a.nchunk * a.fine, (int64_t)a.N * a.Ch, (int64_t)b.n * a.Ch + b.c0 + cw, a.S, q, svec, a.softplus != 0);
     const f32x4 bias = a.dt_bias ? load4n<float, false>(a.dt_bias + b.c0 + lc, ln) : zero;
     const f32x4 Dv = a.D ? load4n<float, false>(a.D + b.c0 + lc, ln) : zero;
     f32x4 dD = zero, dbias = zero;

@@ -38,7 +38,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanDev a, float* __restr
         }
     }
     if (on && blockIdx.y > 0)
-        scan_fold<NG, false>(h, A2, ends, sums, blockIdx.y, a.nchunk, (int64_t)a.N * a.Ch, (int64_t)b.n * a.Ch + b.c0 + cw, a.S, q, svec);
+        scan_fold<NG, false>(h, A2, ends, sums, blockIdx.y, a.nchunk, (int64_t)a.N * a.Ch, (int64_t)b.n * a.Ch + b.c0 + cw, a.S, q, svec, a.softplus != 0);
     const f32x4 bias = a.dt_bias ? load4n<float, false>(a.dt_bias + b.c0 + lc, ln) : f32x4{0.f, 0.f, 0.f, 0.f};
     const f32x4 Dv = a.D ? load4n<float, false>(a.D + b.c0 + lc, ln) : f32x4{0.f, 0.f, 0.f, 0.f};
 

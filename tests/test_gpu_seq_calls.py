@@ -58,3 +58,26 @@ def test_scan_rates_without_memory(ops, rate):
     for name, t in zip(("dx", "ddt", "dB", "dC"), (ins[0], ins[1], ins[3], ins[4])):
         close(name, t.grad, ref[name].view_as(t), mag[name].view_as(t), S + Ch + 60)
     assert not ins[2].grad.any()
+
+
+def test_scan_growth_before_the_signal(ops):
+    """Rates above zero over a silent beginning, long enough that the time axis is split and a chunk's growth passes fp32: zeros stay
+    zeros, and a small state grows to what it is."""
+    T, Ch, S = 1024, 3, 4                                 # one workgroup: split into chunks of 64 frames
+    d, A = 0.5, 5.0                                       # e^2.5 a frame
+    x, B = torch.zeros(T, 1, Ch), torch.ones(T, 1, S)
+    x[1010:] = 1.0
+    dt = torch.full((T, 1, Ch), d)
+    rates = torch.full((Ch, S), A)
+    ref, mag = (seq.scan(x, dt, rates, B, B, softplus=False, mag=m) for m in (False, True))
+    y = ops.ssm_scan(*map(dev, (x, dt, rates, B, B)), softplus=False)
+    close("y", y, ref["y"], mag["y"], 14 * 8 + 20)        # per frame a few roundings of the exponent, 2.5 exp and the sum
+    # backwards: the gradient of the frames behind the loss is zero, however much they would grow
+    dy = torch.zeros(T, 1, Ch)
+    dy[:10] = 1.0
+    x = torch.zeros(T, 1, Ch)
+    ref, mag = (seq.scan(x, dt, rates, B, B, softplus=False, dy=dy, mag=m) for m in (False, True))
+    ins = leaves(x, dt, rates, B, B)
+    ops.ssm_scan(*ins, softplus=False).backward(dev(dy))
+    for name, t in zip(("dx", "ddt", "dA", "dB", "dC"), ins):
+        close(name, t.grad, ref[name].view_as(t), mag[name].view_as(t), 10 * 8 + 20)
