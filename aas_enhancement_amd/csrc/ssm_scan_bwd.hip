@@ -217,12 +217,12 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanDev a, const T* __res
                 vz[i] = gz[i] * fmaf(Dv[i], xe[i], o[i]);
                 dD[i] = fmaf(oe[i], xe[i], dD[i]);
             }
-            vt = cols.keep(vt, live);
+            vt = cols.keep(vt, live);                     // (zeros behind the end also where the row's state has overflowed: 0 inf is none)
             dbias += vt;
             const int64_t at = t * orow + obase;
-            store4n<T, VEC>(dx + at, vx, ln);
+            store4n<T, VEC>(dx + at, cols.keep(vx, live), ln);
             store4n<T, VEC>(ddt + at, vt, ln);
-            if (dz) store4n<T, VEC>(dz + at, vz, ln);
+            if (dz) store4n<T, VEC>(dz + at, cols.keep(vz, live), ln);
         }
         // partial dB, dC of this workgroup: [T][N][G][nblk][2][S]
 #pragma unroll

@@ -81,3 +81,24 @@ def test_scan_growth_before_the_signal(ops):
     ops.ssm_scan(*ins, softplus=False).backward(dev(dy))
     for name, t in zip(("dx", "ddt", "dA", "dB", "dC"), ins):
         close(name, t.grad, ref[name].view_as(t), mag[name].view_as(t), 10 * 8 + 20)
+
+
+def test_scan_gradients_behind_a_row_whose_state_overflowed(ops):
+    """Frames behind a row's end have zero gradients, whatever became of the row; the other rows know nothing of it."""
+    T, N, Ch, S = 40, 2, 4, 3
+    g = torch.Generator().manual_seed(4)
+    x, dt, B, C, z, dy = (rnd(g, T, N, n) for n in (Ch, Ch, S, S, Ch, Ch))
+    A = -torch.ones(Ch, S)
+    n = torch.tensor([5, 40], dtype=torch.int32)
+    ref = seq.scan(x[:, 1:], dt[:, 1:], A, B[:, 1:], C[:, 1:], z=z[:, 1:], dy=dy[:, 1:])
+    mag = seq.scan(x[:, 1:], dt[:, 1:], A, B[:, 1:], C[:, 1:], z=z[:, 1:], dy=dy[:, 1:], mag=True)
+    x[:5, 0], B[:5, 0] = 1e30, 1e30
+    ins = leaves(x, dt, A, B, C)
+    zz, = leaves(z)
+    y = ops.ssm_scan(*ins, z=zz, lengths=dev(n))
+    y.backward(dev(dy))
+    assert not torch.isfinite(y[:5, 0]).all() and not y[5:, 0].any()
+    for t in (ins[0], ins[1], ins[3], ins[4], zz):
+        assert not t.grad[5:, 0].any()
+    for name, t in (("dx", ins[0]), ("ddt", ins[1]), ("dB", ins[3]), ("dC", ins[4]), ("dz", zz)):
+        close(name, t.grad[:, 1:], ref[name].view_as(t[:, 1:]), mag[name].view_as(t[:, 1:]), 2 * (T * 16 + S + 64) + Ch)
