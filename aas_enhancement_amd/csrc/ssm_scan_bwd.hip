@@ -342,7 +342,19 @@ extern "C" int aas_ssm_scan_bwd(aasStream_t stream, const aasScan* d, const void
     if (scan_check(who, d)) return 1;
     hipStream_t s = (hipStream_t)stream;
     const bool empty = d->T == 0 || d->N == 0;
-    if (d->Ch == 0) return 0;
+    const int64_t want = ((int64_t)d->T * d->N * d->G * 2 * d->S + 255) / 256;
+    const int nbc = (int)(want < 8192 ? want : 8192);
+    if (d->Ch == 0) {                                     // dB and dC are the sums of no channels
+        if (empty) return 0;
+        AAS_CHECK(dB && dC, "%s: null pointer", who);
+        ScanDev a;
+        scan_dev(d, &a);
+        const ColMap none = {};
+        AAS_DT_SWITCH(d->dtype, E, hipLaunchKernelGGL(scan_finish_kernel<E>, dim3(nbc), dim3(256), 0, s, a, (const float*)nullptr, (const float*)nullptr,
+                                                      (const float*)nullptr, 0, nbc, 0, (E*)dB, (E*)dC, none, none));
+        AAS_LAUNCH_CHECK(who);
+        return 0;
+    }
     AAS_CHECK(dA != nullptr, "%s: null pointer", who);
     if (!empty) {
         const BwdWs w = bwd_ws(d->T, d->N, d->Ch, d->S, d->G);
@@ -364,8 +376,7 @@ extern "C" int aas_ssm_scan_bwd(aasStream_t stream, const aasScan* d, const void
         AAS_LAUNCH_CHECK(who);
         const ColMap ma = {{dA, nullptr, nullptr, nullptr}, {d->Ch * d->S, 0, 0, 0}, 0, 1};
         const ColMap md = {{dD, ddt_bias, nullptr, nullptr}, {d->Ch, d->Ch, 0, 0}, 0, 2};
-        const int64_t want = ((int64_t)d->T * d->N * d->G * 2 * d->S + 255) / 256;
-        const int nbc = (int)(want < 8192 ? want : 8192), na = cdiv((int64_t)d->Ch * d->S, 16), nd = dD || ddt_bias ? cdiv(2 * (int64_t)d->Ch, 16) : 0;
+        const int na = cdiv((int64_t)d->Ch * d->S, 16), nd = dD || ddt_bias ? cdiv(2 * (int64_t)d->Ch, 16) : 0;
         AAS_DT_SWITCH(d->dtype, E, hipLaunchKernelGGL(scan_finish_kernel<E>, dim3(nbc + na + nd), dim3(256), 0, s, a, (const float*)(base + w.bc),
                                                       (const float*)(base + w.a), (const float*)(base + w.d), d->N * ck.n, nbc, na, (E*)dB, (E*)dC, ma, md));
         AAS_LAUNCH_CHECK(who);

@@ -102,3 +102,16 @@ def test_scan_gradients_behind_a_row_whose_state_overflowed(ops):
         assert not t.grad[5:, 0].any()
     for name, t in (("dx", ins[0]), ("ddt", ins[1]), ("dB", ins[3]), ("dC", ins[4]), ("dz", zz)):
         close(name, t.grad[:, 1:], ref[name].view_as(t[:, 1:]), mag[name].view_as(t[:, 1:]), 2 * (T * 16 + S + 64) + Ch)
+
+
+def test_scan_of_no_channels(ops):
+    """B and C get gradients of zero, not what the memory held."""
+    A = torch.zeros(0, 4, device="cuda", requires_grad=True)
+    x = torch.zeros(3, 2, 0, device="cuda", requires_grad=True)
+    B = torch.ones(3, 2, 4, device="cuda", requires_grad=True)
+    C = torch.ones(3, 2, 4, device="cuda", requires_grad=True)
+    for _ in range(3):
+        full = torch.full((3, 2, 1, 4), 7.0, device="cuda")      # (the block that the gradients are likely to be given)
+        del full
+        dB, dC, dA = torch.autograd.grad(ops.ssm_scan(x, x, A, B, C), (B, C, A), torch.zeros(3, 2, 0, device="cuda"))
+        assert not dB.any() and not dC.any() and dA.shape == (0, 4)
