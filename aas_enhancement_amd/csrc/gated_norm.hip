@@ -142,7 +142,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void gated_bwd_kernel(int64_
 int gated_blocks(int64_t R, int C, int groups, int most) { return norm_blocks(R, C / groups, groups >= most ? 1 : most / groups); }
 constexpr int FWD_MOST = 2048, BWD_MOST = 1024;
 
-bool gated_args(const char* who, int dtype, int64_t R, int C, int groups) {
+bool gated_args(const char* who, int dtype, int64_t R, int C, int groups, float eps) {
+    if (!norm_eps_ok(eps)) { aas_set_error("%s: eps = %g", who, eps); return false; }
     if (!aas_dt_ok(dtype)) { aas_set_error("%s: dtype %d", who, dtype); return false; }
     if (R < 0 || C < 1 || groups < 1 || C % groups) { aas_set_error("%s: R = %lld, C = %d, groups = %d", who, (long long)R, C, groups); return false; }
     if (C / groups > NORM_MAX_C) { aas_set_error("%s: %d channels a group, at most %d", who, C / groups, NORM_MAX_C); return false; }
@@ -155,7 +156,7 @@ bool gated_args(const char* who, int dtype, int64_t R, int C, int groups) {
 extern "C" int aas_gated_norm_fwd(aasStream_t stream, int dtype, int64_t R, int C, int groups, const void* x, int64_t x_ld, const void* gate,
                                   int64_t gate_ld, const float* weight, float eps, int norm_first, void* y) {
     const char* who = "aas_gated_norm_fwd";
-    if (!gated_args(who, dtype, R, C, groups)) return 1;
+    if (!gated_args(who, dtype, R, C, groups, eps)) return 1;
     if (R == 0) return 0;
     AAS_CHECK(x && gate && y, "%s: null pointer", who);
     const int es = aas_dt_size(dtype), cg = C / groups;
@@ -182,7 +183,7 @@ extern "C" int aas_gated_norm_bwd(aasStream_t stream, int dtype, int64_t R, int 
                                   const void* gate, int64_t gate_ld, const float* weight, float eps, int norm_first, void* dx, void* dgate,
                                   float* dweight, void* ws) {
     const char* who = "aas_gated_norm_bwd";
-    if (!gated_args(who, dtype, R, C, groups)) return 1;
+    if (!gated_args(who, dtype, R, C, groups, eps)) return 1;
     // (the launch that sums dweight has a workgroup of 256 per 16 columns, and fewer than 2^32 threads)
     AAS_CHECK(!dweight || cdiv(C, 16) < (1 << 24), "%s: C = %d too large for a weight's gradient", who, C);
     hipStream_t s = (hipStream_t)stream;

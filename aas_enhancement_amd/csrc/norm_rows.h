@@ -97,3 +97,4 @@ static inline int norm_blocks(int64_t rows, int C, int most) {
     const int64_t groups = C <= 1024 ? (rows + 3) / 4 : rows;
     return (int)(groups < most ? (groups < 1 ? 1 : groups) : most);
 }
+static inline bool norm_eps_ok(float eps) { return eps >= 0.f && eps <= 3.4028234e38f; }

@@ -202,6 +202,7 @@ extern "C" int aas_residual_norm_fwd(aasStream_t stream, int dtype, int r_dtype,
                                      int64_t seed, int64_t offset, const int64_t* d_seed, int64_t* seed_used, void* y, void* r, float* stat) {
     const char* who = "aas_residual_norm_fwd";
     if (!norm_args(who, dtype, r_dtype, R, C, thr)) return 1;
+    AAS_CHECK(norm_eps_ok(eps), "%s: eps = %g", who, eps);
     if (R == 0) return 0;
     AAS_CHECK(x && y, "%s: null pointer", who);
     AAS_CHECK(r || (!residual && !scale && !thr && r_dtype == dtype), "%s: r is wanted", who);

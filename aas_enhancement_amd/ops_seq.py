@@ -160,6 +160,13 @@ def _whole(*ts):
     return [t if t is None or t.is_contiguous() else t.contiguous() for t in ts]
 
 
+def _eps(who, eps):
+    eps = float(eps)
+    if not 0.0 <= eps < math.inf:
+        _bad(who, "eps must be a number from 0 on, got %r" % (eps,))
+    return eps
+
+
 def _rows(t):
     """-> (tensor, row pitch): the leading dimensions as uniformly spaced rows, copied where they are not."""
     t = _unit(t)
@@ -496,7 +503,7 @@ def residual_norm(x, residual=None, weight=None, bias=None, scale=None, eps=1e-5
         residual = _activation(who, "residual", residual)
     weight, bias, scale = (_param(who, n, t, x, (C,)) for n, t in (("weight", weight), ("bias", bias), ("scale", scale)))
     drop = _drop_args(who, x, p, seed, offset)
-    eps, layer = float(eps), 1 if kind == "layer" else 0
+    eps, layer = _eps(who, eps), 1 if kind == "layer" else 0
     if residual is None and scale is None and not drop[0]:
         if _wants_grad(x, weight, bias):
             return _Norm.apply(x, None, weight, bias, None, eps, layer, drop)
@@ -557,7 +564,7 @@ def gated_norm(x, gate, weight=None, eps=1e-5, groups=1, norm_first=False):
     if groups < 1 or C % groups or C // groups > 16384:
         _bad(who, "%d channels do not divide into %d groups of at most 16384" % (C, groups))
     weight = _param(who, "weight", weight, x, (C,))
-    eps, norm_first = float(eps), 1 if norm_first else 0
+    eps, norm_first = _eps(who, eps), 1 if norm_first else 0
     if _wants_grad(x, gate, weight):
         return _GatedNorm.apply(x, gate, weight, eps, groups, norm_first)
     (xr, x_ld), (gr, g_ld) = _rows(x), _rows(gate)

@@ -580,7 +580,7 @@ int aas_ssm_scan_bwd(aasStream_t stream, const aasScan* d, const void* dy, int64
 
 /* Residual sum and the norm in front of the next block, one pass (C <= 16384):
  *   r = residual + scale * drop(x)  (kept in r_dtype: dtype or AAS_DT_F32),   y = (r - mean) rstd weight + bias,
- * with mean over the row (layer = 1) or 0 (layer = 0), rstd = 1 / sqrt(mean((r - mean)^2) + eps); the norm reads r as it is kept.
+ * with mean over the row (layer = 1) or 0 (layer = 0), rstd = 1 / sqrt(mean((r - mean)^2) + eps), eps >= 0; the norm reads r as it is kept.
  * residual, weight, bias, scale may be NULL (zeros, ones, zeros, ones; without residual, scale and dropout r may be NULL: it is x).
  * Dropout: element i of x in row-major order is kept iff its 16 random bits are >= thr (0 <= thr <= 65536; 0 = no dropout), a kept one
  * is multiplied by 65536 / (65536 - thr).  The bits: counter offset + i / 8 of Philox-4x32-10 (Salmon et al. 2011) under the key `seed`,
@@ -599,7 +599,7 @@ int aas_residual_norm_bwd(aasStream_t stream, int dtype, int r_dtype, int64_t R,
                           void* dresidual, float* dweight, float* dbias, float* dscale, void* ws);
 
 /* Root-mean-square norm behind a block with its gate, per group of C / groups channels (<= 16384 channels a group):
- *   norm_first = 0: y = norm(x silu(gate)) weight;   norm_first = 1: y = norm(x) weight silu(gate),   norm(v) = v / sqrt(mean(v^2) + eps).
+ *   norm_first = 0: y = norm(x silu(gate)) weight;   norm_first = 1: y = norm(x) weight silu(gate),   norm(v) = v / sqrt(mean(v^2) + eps), eps >= 0.
  * x, gate: R rows of pitch x_ld, gate_ld; weight [C] may be NULL (ones). */
 int aas_gated_norm_fwd(aasStream_t stream, int dtype, int64_t R, int C, int groups, const void* x, int64_t x_ld, const void* gate,
                        int64_t gate_ld, const float* weight, float eps, int norm_first, void* y);

@@ -180,3 +180,20 @@ def test_gated_norm_c_entry_refuses_rows_times_groups_past_64_bits():
     L = _lib.lib()
     _refuses(L.aas_gated_norm_fwd(None, 0, 1 << 62, 16, 4, None, 16, one, 16, None, 1e-5, 0, one), b"too large")
     _refuses(L.aas_gated_norm_bwd(None, 0, 1 << 62, 16, 4, None, 16, one, 16, one, 16, None, 1e-5, 0, one, one, None, None), b"too large")
+
+
+def test_norms_refuse_eps_outside_the_numbers_it_may_be(door):
+    """A negative one makes the root of a negative number, a NaN or an infinite one wipes every row out."""
+    x = torch.randn(4, 8)
+    for eps in (-1e-5, float("nan"), float("inf")):
+        for f in (lambda: ops_seq.residual_norm(x, eps=eps), lambda: ops_seq.gated_norm(x, x, eps=eps)):
+            with pytest.raises(RuntimeError, match="eps must be"):
+                f()
+    for eps in (0.0, 0, 1e-12, 1.0):
+        ops_seq.residual_norm(x, eps=eps)
+        ops_seq.gated_norm(x, x, eps=eps)
+    one, L = 4096, _lib.lib()      # (pointers that are missing end the calls in any case)
+    for eps in (-1e-5, float("nan"), float("inf")):
+        _refuses(L.aas_residual_norm_fwd(None, 0, 0, 1, 8, None, 8, None, 0, None, None, None, eps, 0, 0, 0, 0, None, None, one, one, None), b"eps")
+        _refuses(L.aas_gated_norm_fwd(None, 0, 1, 8, 1, None, 8, one, 8, None, eps, 0, one), b"eps")
+        _refuses(L.aas_gated_norm_bwd(None, 0, 1, 8, 1, None, 8, one, 8, one, 8, None, eps, 0, one, one, None, None), b"eps")
