@@ -57,6 +57,29 @@ template <int TPR> __device__ __forceinline__ void row_sum2(float& a, float& b, 
     }
 }
 
+// Rows whose squares leave fp32's range are summed once more, scaled by a power of two (the same answer for all of a row's threads).  Below
+// a mean square of 2^-100 (eps = 0: a larger eps holds it up) squares lose bits that count and the hardware root takes a denormal for
+// zero; at infinity they have overflowed.  2^76 up brings the former to 2^-124 .. 2^52 in size, 2^76 down a row of finite numbers
+// (2^128 at most, 2^57 or more if its squares overflow over 16384 columns) inside as well.  0: an ordinary row, or one that holds a NaN.
+constexpr float ROW_SMALL = 0x1p-100f, ROW_UP = 0x1p76f, ROW_DOWN = 0x1p-76f;
+__device__ __forceinline__ float row_rescale(float ms) { return ms < ROW_SMALL ? ROW_UP : ms > 3.4028234e38f ? ROW_DOWN : 0.f; }
+
+// 1 / sqrt(mean(v^2) + eps) from the sum of the squares
+template <int TPR, int NV> __device__ __forceinline__ float row_rstd(const f32x4 (&v)[NV], float sum, float inv, float eps, float (*s)[2]) {
+    const float ms = fmaf(sum, inv, eps), c = row_rescale(ms);
+    if (c == 0.f) return __builtin_amdgcn_rsqf(ms);
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float u = v[i][j] * c;
+            s1 = fmaf(u, u, s1);
+        }
+    row_sum2<TPR>(s1, s2, s);
+    return __builtin_amdgcn_rsqf(fmaf(s1, inv, eps * c * c)) * c;
+}
+
 // the column sums acc[i] (quad i) of a workgroup's rows -> out[0 .. C); four rows a workgroup are joined through LDS
 template <int TPR, int NV> __device__ __forceinline__ void put_columns(const f32x4* acc, float* out, int C, float* lds) {
     const int l = threadIdx.x % TPR, r = threadIdx.x / TPR;

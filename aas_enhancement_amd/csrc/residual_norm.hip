@@ -12,8 +12,12 @@ namespace {
 
 struct Drop { unsigned thr; float factor; int64_t seed, offset; const int64_t* d_seed; };
 
+// Rows of 513 to 1024 columns all in 16 bits are held to six waves a SIMD: left alone they take two registers more than those have, and
+// 16384 x 1000 takes 27.2 us instead of 26.3.
+template <class R, int TPR, int NV, bool VEC> constexpr int residual_fwd_waves() { return sizeof(R) == 2 && NV == 4 && TPR == 64 && VEC ? 6 : 1; }
+
 template <class T, class R, int TPR, int NV, bool VEC>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_fwd_kernel(int64_t rows, int C, const T* __restrict__ x, int64_t x_ld,
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256, (residual_fwd_waves<R, TPR, NV, VEC>())) void residual_fwd_kernel(int64_t rows, int C, const T* __restrict__ x, int64_t x_ld,
                                                                               const R* __restrict__ res, int64_t res_ld, const float* __restrict__ w,
                                                                               const float* __restrict__ b, const float* __restrict__ sc, float eps, int layer,
                                                                               Drop dr, int64_t* __restrict__ used, T* __restrict__ y, R* __restrict__ r_out,
@@ -68,7 +72,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_fwd_kernel(int
                 s1 = fmaf(v[i][j], v[i][j], s1);
             }
         row_sum2<TPR>(s1, s2, s);
-        const float rstd = __builtin_amdgcn_rsqf(fmaf(s1, inv, eps));
+        const float rstd = row_rstd<TPR>(v, s1, inv, eps, s);
         if (stat && l == 0) {
             stat[2 * row] = mean;
             stat[2 * row + 1] = rstd;

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from oracle import seq
-from tests.test_gpu_seq import close, dev, leaves, ops, rnd  # noqa: F401
+from tests.test_gpu_seq import IDS, U, close, dev, leaves, ops, rnd  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -115,3 +115,46 @@ def test_scan_of_no_channels(ops):
         del full
         dB, dC, dA = torch.autograd.grad(ops.ssm_scan(x, x, A, B, C), (B, C, A), torch.zeros(3, 2, 0, device="cuda"))
         assert not dB.any() and not dC.any() and dA.shape == (0, 4)
+
+
+# ------------------------------------------------------------------------------------------------- norms: rows far from one in size
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=IDS.get)
+@pytest.mark.parametrize("C", [12, 13, 700, 1500, 1501, 4096, 9000])
+def test_norms_of_rows_whose_squares_leave_fp32(ops, C, dtype):
+    """Rows of 1e-36 to 1e30 in one call, among them ordinary ones: the squares underflow (with eps = 0) or overflow, the norms do not.
+    Tolerances as for ordinary rows: 200 roundings of the largest value's share."""
+    sizes = [1.0, 1e-18, 1e-21, 1e-30, 1e-36, 3e18, 1e25, 1e30, 2.0]
+    g = torch.Generator().manual_seed(C)
+    R, k = len(sizes), 220
+    scale = torch.tensor(sizes).unsqueeze(1)
+    x, z, w, dy = (rnd(g, R, C) * scale).to(dtype), rnd(g, R, C, dtype=dtype), rnd(g, C, mean=1.0, std=0.3), rnd(g, R, C, dtype=dtype)
+    top = lambda v: v.abs().amax(-1, keepdim=True)     # noqa: E731
+    for eps in (0.0, 1e-5):
+        for kind in ("rms", "layer"):
+            ref = seq.residual_norm(x, weight=w, eps=eps, kind=kind, dy=dy)
+            xx, ww = leaves(x, w)
+            y, _ = ops.residual_norm(xx, weight=ww, eps=eps, kind=kind)
+            y.backward(dev(dy))
+            v = x.double()
+            v = v - v.mean(-1, keepdim=True) if kind == "layer" else v
+            rstd = 1 / torch.sqrt(v.square().mean(-1, keepdim=True) + eps)
+            hm, gm = top(x.double()) * rstd, top(dy.double() * w.double())
+            close("y", y, ref["y"], hm * w.double().abs() * (1 + hm * hm * (kind == "layer")), k)
+            close("dx", xx.grad, ref["dx"], rstd * gm * (2 + 2 * hm * hm) * (1 + hm * hm), k)
+            close("dw", ww.grad, ref["dweight"], (dy.double().abs() * hm * (1 + hm * hm)).sum(0), k + R)
+        for first in (False, True):
+            ref = seq.gated_norm(x, z, w, eps, 1, first, dy)
+            xx, zz, ww = leaves(x, z, w)
+            y = ops.gated_norm(xx, zz, ww, eps=eps, norm_first=first)
+            y.backward(dev(dy))
+            gt = z.double() * torch.sigmoid(z.double())
+            v = x.double() if first else x.double() * gt
+            rstd = 1 / torch.sqrt(v.square().mean(-1, keepdim=True) + eps)
+            # (x silu(gate) is a product in fp32: below 2^-126 a multiple of 2^-149, off by up to 2^-150 whatever its size)
+            lost = 0.0 if first else 2.0 ** -150 / (k * U)
+            hm, gm, out = (v.abs() + lost) * rstd, dy.double().abs() * w.double().abs() * (gt.abs() if first else 1), gt.abs() if first else 1
+            dvm = rstd * (gm + top(hm) * top(gm) * top(hm))
+            close("y", y, ref["y"], hm * w.double().abs() * out, k)
+            close("dx", xx.grad, ref["dx"], dvm if first else dvm * gt.abs(), k)
+            close("dgate", zz.grad, ref["dgate"], dy.double().abs() * hm * w.double().abs() * 1.2 if first else dvm * x.double().abs() * 1.2, k)
+            close("dw", ww.grad, ref["dweight"], (dy.double().abs() * hm * out).sum(0), k + R)
