@@ -158,3 +158,132 @@ def test_norms_of_rows_whose_squares_leave_fp32(ops, C, dtype):
             close("dx", xx.grad, ref["dx"], dvm if first else dvm * gt.abs(), k)
             close("dgate", zz.grad, ref["dgate"], dy.double().abs() * hm * w.double().abs() * 1.2 if first else dvm * x.double().abs() * 1.2, k)
             close("dw", ww.grad, ref["dweight"], (dy.double().abs() * hm * out).sum(0), k + R)
+
+
+# --------------------------------------------------------------------------------------------- states in graphs, two threads, far offsets
+def _stream_step(ops, p):
+    def step(x, res, cs, ss):
+        y, r = ops.residual_norm(x, res, p["w"])
+        u = ops.causal_conv1d(y, p["cw"], state=cs)
+        h = ops.ssm_scan(u, y, p["A"], y[..., :16], y[..., 4:20], D=p["w"], state=ss)
+        return ops.gated_norm(h, y, p["w"]), r
+    return step
+
+
+def test_single_frames_and_prompts_replayed_from_graphs(ops):
+    """The states are read and written in place by every replay: a frame at a time, and a prompt whose time axis is split."""
+    g = torch.Generator().manual_seed(20)
+    C, N = 24, 2
+    p = dict(w=rnd(g, C, mean=1.0, std=0.1).cuda(), cw=rnd(g, C, 4).cuda(), A=-torch.rand(C, 16).cuda() - 0.1)
+    step = _stream_step(ops, p)
+    with torch.no_grad():
+        for T in (1, 300):
+            x, res = torch.zeros(T, N, C, device="cuda"), torch.zeros(T, N, C, device="cuda")
+            cs, ss = torch.zeros(N, 3, C, device="cuda"), torch.zeros(N, C, 16, device="cuda")
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                step(x, res, cs, ss)
+            torch.cuda.current_stream().wait_stream(side)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = step(x, res, cs, ss)
+            c2, s2 = rnd(g, N, 3, C).cuda(), rnd(g, N, C, 16).cuda()
+            cs.copy_(c2)
+            ss.copy_(s2)
+            for _ in range(5):
+                x.copy_(rnd(g, T, N, C))
+                res.copy_(rnd(g, T, N, C))
+                graph.replay()
+                torch.cuda.synchronize()
+                got = [v.clone() for v in out]
+                want = step(x, res, c2, s2)
+                for a, b in zip(got + [cs, ss], list(want) + [c2, s2]):
+                    assert torch.equal(a, b)
+
+
+def test_two_threads_on_their_own_streams(ops):
+    """Each thread's training steps give what they give alone."""
+    import threading
+
+    def work(seed, stream, out):
+        with torch.cuda.stream(stream):
+            g = torch.Generator().manual_seed(seed)
+            T, N, C = 90, 2, 40 + 8 * seed
+            for _ in range(6):
+                x, z, dy = (rnd(g, T, N, C).cuda().requires_grad_(i < 2) for i in range(3))
+                A, B, w = (-torch.ones(C, 16)).cuda().requires_grad_(), rnd(g, T, N, 16).cuda().requires_grad_(), rnd(g, C, mean=1.0).cuda().requires_grad_()
+                y = ops.ssm_scan(ops.causal_conv1d(x, rnd(g, C, 4).cuda()), z, A, B, B, z=z)
+                y, r = ops.residual_norm(ops.gated_norm(y, z, w), ops.dropout(x, 0.2, seed), w, p=0.1, seed=seed)
+                out.append([t.clone() for t in (y, r) + torch.autograd.grad((y, r), (x, z, A, B, w), (dy, dy))])
+            stream.synchronize()
+    alone, both, streams = [[], []], [[], []], [torch.cuda.Stream() for _ in range(2)]
+    for k in range(2):
+        work(k, streams[k], alone[k])
+    threads = [threading.Thread(target=work, args=(k, streams[k], both[k])) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k in range(2):
+        assert len(both[k]) == 6
+        for a, b in zip(alone[k], both[k]):
+            for u, v in zip(a, b):
+                assert torch.equal(u, v)
+
+
+def test_rows_far_apart(ops):
+    """Views whose offsets pass 2^31 elements: three frames of two rows, spread over one allocation."""
+    g = torch.Generator().manual_seed(21)
+    T, N, C, far, row = 3, 2, 8, 900_000_000, 400_000_000
+    room = torch.empty(2 * far + row + 128, dtype=torch.bfloat16, device="cuda")
+
+    def spread(t, at):
+        v = room.as_strided(t.shape, (far, row) + t.stride()[2:], at)
+        v.copy_(t)
+        return v
+    x, dt, z, B, dy = (rnd(g, T, N, n, dtype=torch.bfloat16).cuda() for n in (C, C, C, 16, C))
+    w, A, v = rnd(g, C, 4).cuda(), -torch.ones(C, 16, device="cuda"), rnd(g, C, mean=1.0).cuda()
+
+    def grads(x, dt, z, B, dy):
+        ins = [t.detach().requires_grad_() for t in (x, dt, z, B)]
+        ps = [t.detach().clone().requires_grad_() for t in (w, A, v)]
+        outs = [ops.causal_conv1d(ins[0], ps[0]), ops.ssm_scan(ins[0], ins[1], ps[1], ins[3], ins[3], D=ps[2], z=ins[2])]
+        rows = [ins[0][:, 0], ins[2][:, 1]]                # a row pitch of `far`
+        y, r = ops.residual_norm(*rows, ps[2], scale=ps[2])
+        outs += [y, r, ops.gated_norm(*rows, ps[2])]
+        got = torch.autograd.grad(outs, ps, [dy, dy] + [dy[:, 0]] * 3, retain_graph=True)
+        return outs + list(got)
+    near = grads(x, dt, z, B, dy)
+    away = grads(*(spread(t, 16 * i) for i, t in enumerate((x, dt, z, B, dy))))
+    for a, b in zip(near, away):
+        assert torch.equal(a, b)
+
+
+def test_more_than_2_to_the_31_elements(ops):
+    """Outputs past 32-bit offsets: the last rows of a large call are what they are in a small one."""
+    def tail(f, n):
+        whole, part = f(slice(None)), f(slice(-n, None))
+        for a, b in zip(whole, part):
+            a = a[-n:] if a.shape[0] != b.shape[0] else a
+            assert torch.equal(a, b)
+    R, C = 2 ** 21 + 5, 1032
+    x = torch.randn(R, C, device="cuda", dtype=torch.bfloat16)
+    w = torch.rand(C, device="cuda")
+    tail(lambda s: ops.residual_norm(x[s], x[s], w), 9)
+    tail(lambda s: (ops.gated_norm(x[s], x[s], w),), 9)
+    off = (R - 16) * C // 8
+    assert torch.equal(ops.dropout(x, 0.4, 3)[-16:], ops.dropout(x[-16:], 0.4, 3, off))
+    T, N = 2 ** 16, 32
+    v = x[:T * N].view(T, N, C)
+    k = torch.rand(C, 4, device="cuda")
+    a = ops.causal_conv1d(v, k)
+    assert torch.equal(a[-20:], ops.causal_conv1d(v[-23:], k)[3:])
+    del a
+    # the scan, rows last: every row is on its own
+    s, A = v.view(2048, 1024, C), -torch.ones(C, 4, device="cuda")
+    B = torch.randn(2048, 1024, 4, device="cuda", dtype=torch.bfloat16)
+    a = ops.ssm_scan(s, s, A, B, B, z=s)
+    b = ops.ssm_scan(s[:, -300:], s[:, -300:], A, B[:, -300:], B[:, -300:], z=s[:, -300:])     # (enough rows to be unsplit, too)
+    assert torch.equal(a[:, -300:], b)
