@@ -20,6 +20,7 @@ _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # include/aas_
 
 _raw_stream = torch._C._cuda_getCurrentRawStream     # what torch.cuda.current_stream().cuda_stream ends in, without the object (3-6 us a call)
 _empty = torch.empty
+_INF = math.inf
 
 # include/aas_hip.h: aasScan, as packed bytes (a ctypes.Structure of 36 fields takes 3 us longer to fill)
 _SCAN_FIELDS = (["size", "dtype", "T", "N", "Ch", "S", "G", "softplus"], ["x", "dt", "z", "B", "C", "A", "D", "dt_bias", "len"],
@@ -160,18 +161,12 @@ def _whole(*ts):
     return [t if t is None or t.is_contiguous() else t.contiguous() for t in ts]
 
 
-def _eps(who, eps):
-    eps = float(eps)
-    if not 0.0 <= eps < math.inf:
-        _bad(who, "eps must be a number from 0 on, got %r" % (eps,))
-    return eps
-
-
 def _rows(t):
     """-> (tensor, row pitch): the leading dimensions as uniformly spaced rows, copied where they are not."""
-    t = _unit(t)
     if t.is_contiguous():
         return t, t.shape[-1]
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        return t.contiguous(), t.shape[-1]
     pitch, seen = None, 1
     for size, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
         if size == 1:
@@ -503,7 +498,9 @@ def residual_norm(x, residual=None, weight=None, bias=None, scale=None, eps=1e-5
         residual = _activation(who, "residual", residual)
     weight, bias, scale = (_param(who, n, t, x, (C,)) for n, t in (("weight", weight), ("bias", bias), ("scale", scale)))
     drop = _drop_args(who, x, p, seed, offset)
-    eps, layer = _eps(who, eps), 1 if kind == "layer" else 0
+    eps, layer = float(eps), 1 if kind == "layer" else 0
+    if not 0.0 <= eps < _INF:
+        _bad(who, "eps must be a number from 0 on, got %r" % (eps,))
     if residual is None and scale is None and not drop[0]:
         if _wants_grad(x, weight, bias):
             return _Norm.apply(x, None, weight, bias, None, eps, layer, drop)
@@ -564,7 +561,9 @@ def gated_norm(x, gate, weight=None, eps=1e-5, groups=1, norm_first=False):
     if groups < 1 or C % groups or C // groups > 16384:
         _bad(who, "%d channels do not divide into %d groups of at most 16384" % (C, groups))
     weight = _param(who, "weight", weight, x, (C,))
-    eps, norm_first = _eps(who, eps), 1 if norm_first else 0
+    eps, norm_first = float(eps), 1 if norm_first else 0
+    if not 0.0 <= eps < _INF:
+        _bad(who, "eps must be a number from 0 on, got %r" % (eps,))
     if _wants_grad(x, gate, weight):
         return _GatedNorm.apply(x, gate, weight, eps, groups, norm_first)
     (xr, x_ld), (gr, g_ld) = _rows(x), _rows(gate)
