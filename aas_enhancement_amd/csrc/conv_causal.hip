@@ -6,7 +6,10 @@
 //
 // HBM-bound: x in, y out (backward: x and dy in, dx out).  A thread owns four neighbouring channels and runs over a stretch of the time
 // axis with the K frames of its window in registers, so each element is read once plus K - 1 frames of overlap per stretch; lanes
-// run along channels, then rows, then stretches.  4096 x 4 x 2048, K = 4, forward / backward: 28 / 80 us in bf16, 46 / 106 in fp32.
+// run along channels, then rows, then stretches.  4096 x 4 x 2048, K = 4, forward / backward: 27 / 81 us in bf16 (4.9 / 2.5
+// TB/s of x, dy and dx), 50 / 101 in fp32.  The backward kernel is held to four waves a SIMD (128 registers): with K = 4 its fp32 and its element-wise
+// forms spill 3 and 8 of them.  Where C is small and T large the launch that joins the partial rows has few workgroups and decides: 4096 x 32 x 16
+// 50 us backward, 2000 x 32 x 80 43.
 #include "seq_common.h"
 
 namespace {

@@ -2,7 +2,8 @@
 //   norm_first = 0: v = x G, y = hat w;      norm_first = 1: v = x, y = hat w G;      hat = v rstd, rstd = 1 / sqrt(mean(v^2) + eps);
 //   g = dy w (G),  dv = rstd (g - hat mean(g hat));   dx = dv G, dz = dv x G', dw = sum dy hat   |   dx = dv, dz = dy hat w G', dw = sum dy hat G.
 // HBM-bound: every tensor once; the backward pass forms the statistics again from x and z, which it reads anyway.  16384 x 2048 in bf16,
-// forward / backward: 47 / 74 us (4.3 / 4.6 TB/s; without the next row read ahead 52 / 102).
+// forward / backward: 41 / 73 us in 4 groups (4.9 / 4.6 TB/s; without the next row read ahead 52 / 102), 35 / 90 in one; above 8192 channels a group
+// the backward kernel spills 27 to 52 registers: 2048 x 16384 38 / 252.
 #include "norm_rows.h"
 
 namespace {

@@ -59,8 +59,9 @@ template <int TPR> __device__ __forceinline__ void row_sum2(float& a, float& b, 
 
 // Rows whose squares leave fp32's range are summed once more, scaled by a power of two (the same answer for all of a row's threads).  Below
 // a mean square of 2^-100 (eps = 0: a larger eps holds it up) squares lose bits that count and the hardware root takes a denormal for
-// zero; at infinity they have overflowed.  2^76 up brings the former to 2^-124 .. 2^52 in size, 2^76 down a row of finite numbers
-// (2^128 at most, 2^57 or more if its squares overflow over 16384 columns) inside as well.  0: an ordinary row, or one that holds a NaN.
+// zero; at infinity they have overflowed.  2^76 up brings the former's mean squares to 2^-100 .. 2^52 (normal numbers), 2^76 down those of
+// finite numbers (a root mean square of 2^57 or more if the squares overflow over 16384 columns, 2^128 at most) to 2^-38 .. 2^104.  0: an
+// ordinary row, or one that holds a NaN.
 constexpr float ROW_SMALL = 0x1p-100f, ROW_UP = 0x1p76f, ROW_DOWN = 0x1p-76f;
 __device__ __forceinline__ float row_rescale(float ms) { return ms < ROW_SMALL ? ROW_UP : ms > 3.4028234e38f ? ROW_DOWN : 0.f; }
 

@@ -4,7 +4,8 @@
 //   dresidual = dr,  dx = scale drop(dr),  dweight = sum dy hat,  dbias = sum dy,  dscale = sum dr drop(x)   (sums over rows).
 // HBM-bound: every tensor once.  The norm reads r as it is kept (rounded to r's type), which is also what the backward pass reads: the
 // gradient is that of the values that were computed.  The dropout mask is formed again from its counter.  bf16 onto an fp32 residual,
-// forward / backward: 16384 x 1024 38 / 72 us (5.3 / 4.2 TB/s; with dropout 39 / 78), 6000 x 500 11.6 / 16.5.
+// forward / backward: 16384 x 1024 35 / 66 us (5.8 / 4.6 TB/s), 6000 x 500 with scale and dropout 11.2 / 15.6; above 8192 columns the backward kernel
+// spills 120 to 240 registers: 2048 x 16384 87 / 324.
 #include "norm_rows.h"
 #include "philox.h"
 

@@ -1,5 +1,5 @@
-// Shared device helpers of the causal sequence operators (conv_causal.hip, ssm_scan*.hip, norm_rows.hip, dropout.hip): activations in
-// fp32, bf16 or fp16 (type code AAS_DT_*), parameters, states and every sum in fp32.
+// Shared device helpers of the causal sequence operators (conv_causal.hip, ssm_scan*.hip, residual_norm.hip, gated_norm.hip,
+// dropout.hip): activations in fp32, bf16 or fp16 (type code AAS_DT_*), parameters, the scan's states and every sum in fp32.
 #pragma once
 #include "common.h"
 
@@ -37,8 +37,8 @@ template <class T, bool VEC> __device__ __forceinline__ void store4n(T* p, f32x4
     }
 }
 
-// 1 / (1 + e^-x) on the hardware exponential and reciprocal (1 ulp each): relative error below 2e-7 (1 + |x|) on the small side, where the
-// value itself is e^-|x|; 0 and 1 at the infinities, NaN stays
+// 1 / (1 + e^-x) on the hardware exponential and reciprocal (1 ulp each): relative error below 2e-7 (1 + |x|) down to x = -87, where the
+// value is e^x; 0 below that (1 + e^-x passes what the reciprocal of a normal number can hold), 0 and 1 at the infinities, NaN stays
 __device__ __forceinline__ float sigm(float x) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x)); }
 
 // sum over the four lanes of a quad (every lane gets it)

@@ -79,7 +79,7 @@ template <bool VEC> struct ScanCols {
 };
 
 // d = softplus(v) = max(v, 0) + log(1 + e), e = e^-|v|, and its derivative.  log(1 + e) = 2 atanh(e / (2 + e)): the argument s is at most
-// 1/3 and atanh(s) / s a polynomial in s^2 (Chebyshev interpolation, off by 4e-9), so d keeps full relative accuracy where e is tiny (d
+// 1/3 and atanh(s) / s a polynomial in s^2 (Chebyshev interpolation, off by less than 8e-9), so d keeps full relative accuracy where e is tiny (d
 // of 1e-3 and below), which log(1 + e) formed in fp32 has not.  The exponential takes the rounding of v log2(e) along.
 __device__ __forceinline__ float scan_softplus(float v, float* slope) {
     const float a = fabsf(v), m = a > 200.f ? 200.f : a, p = m * SCAN_LOG2E;               // (e is 0 from 104 on; an infinite m would make NaN below)

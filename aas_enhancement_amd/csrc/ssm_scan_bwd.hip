@@ -6,10 +6,11 @@
 //
 // Tiles of 16 frames from the last to the first, in runs of 8: a lane goes forward from the state that the forward pass kept in front of
 // the run, holding a and p of its frames in registers, then back through them.  (States kept every 16 frames and the exponentials
-// formed twice was 289 us where this was 275, at 4096 x 4 x 1024 in bf16; now 263, at 200 x 30 x 1000 in fp32 91.  All 16 frames' a and p
-// do not fit the registers.)  Bound by instruction issue (105 a frame and wave, VALU active in 77 % of the busy cycles) at two waves a
+// formed twice was 289 us where this was 275, at 4096 x 4 x 1024 in bf16; now 258 to 273, at 200 x 30 x 1000 in fp32 95.  All 16 frames' a and p
+// do not fit the registers.)  Bound by instruction issue (105 a frame and wave, VALU active in 79 % of the busy cycles) at two waves a
 // SIMD; held to three by launch bounds it spills: 561 us, and with a thread's own elements parked in LDS, where it nearly fits, three waves
-// were no faster (pass 578 us against 507).  dB and dC are sums over channels: eight values a lane (four
+// were no faster (pass 578 us against 507).  Above 16 states there is one wave a SIMD (256 registers and 8 to 100 more of the accumulators'):
+// 1000 x 8 x 512 in bf16 takes 108, 244 and 450 us with 16, 32 and 64 states.  dB and dC are sums over channels: eight values a lane (four
 // states x {dB, dC}) over the 16 channels of a wave go by exchanges that halve the number of values with the number of lanes still to
 // add (lane halves, rows of 16, then within the row), then over the four waves through LDS, then - plain stores, no atomics - over the
 // workgroups by a second launch.

@@ -1,7 +1,7 @@
 // Selective state space scan, forward (ssm_scan.h has the mathematics and the layout).  Bound by instruction issue (the VALU is active in
-// 91 % of the busy cycles): a frame is 23 instructions a wave for the recurrence of 16 channels x 16 states, four of them exponentials at a
-// quarter of the rate, and 14 for staging and the gate.  2001 x 3 x 1000 in bf16: 18 us carry + 30 us; 4096 x 4 x 1024 with the states kept
-// for the backward pass: 61 + 98 us; 200 x 30 x 1000 unsplit in fp32: 44.
+// 95 % of the busy cycles at 4096 x 4 x 1024): a frame is 23 instructions a wave for the recurrence of 16 channels x 16 states, four of them exponentials at a
+// quarter of the rate, and 14 for staging and the gate.  2001 x 3 x 1000 in bf16: 19 us carry + 31 us; 4096 x 4 x 1024 with the states kept
+// for the backward pass: 59 + 97 us; 200 x 30 x 1000 unsplit in fp32: 42.
 #include "scan_carry.h"
 
 namespace {

@@ -2,10 +2,11 @@
 of a causal residual block, for a network that has to answer frame by frame (the recurrent layers of `ops` read the whole utterance).
 
 Activations are time-major [T, N, C] (or rows [..., C] for the norms and dropout) in fp32, bf16 or fp16 and may be views - a slice of a
-wider projection, a transposed [N, T, C] - as long as the channels are contiguous; anything else is copied.  Parameters, states and
-every sum are fp32.  `lengths` (int32 [N] on the device, values brought into [0, T]) are the frames of each row of a padded batch: what
-lies behind them is not read, its outputs and gradients are zero.  Every call launches on the current stream of its tensors' device,
-may be captured into a graph, and gives the same bits on every run.  Names stand in `ops`: `ops.ssm_scan(...)`.
+wider projection, a transposed [N, T, C] - as long as the channels are contiguous; anything else is copied.  Parameters, the scan's
+state and every sum are fp32, the convolution's state is of x's type.  `lengths` (int32 [N] on the device, values brought into [0, T])
+are the frames of each row of a padded batch: what lies behind them is not read, its outputs and gradients are zero.  Every call
+launches on the current stream of its tensors' device, may be captured into a graph, and gives the same bits on every run.  First
+derivatives in reverse mode only; others raise.  Names stand in `ops`: `ops.ssm_scan(...)`.
 """
 import functools
 import math

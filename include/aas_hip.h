@@ -535,8 +535,8 @@ int aas_lmfb320_fwd(aasStream_t stream, const float* wave, const int* d_lens, in
 /* ---------------------------------------------------------------- causal sequence operators ---
  * The parts of a causal residual block over time-major activations [T, N, C] - what a live (frame by frame) enhancer needs beside the
  * bidirectional layers above, which read the whole utterance.  Types: `dtype` (AAS_DT_*) is that of the activations and of their
- * gradients; parameters, their gradients, states, statistics and every sum are fp32.  Activation INPUTS are views: channel stride 1
- * and element strides (time, row) or a row pitch of the caller's; outputs are contiguous.  `len` (device int32 [N], may be NULL): frames
+ * gradients, and of the convolution's state; parameters, their gradients, the scan's states, statistics and every sum are fp32.
+ * Activation INPUTS are views: channel stride 1 and element strides (time, row) or a row pitch of the caller's; outputs are contiguous.  `len` (device int32 [N], may be NULL): frames
  * of each row of a padded batch, brought into [0, T]; frames behind a row's last one are not read into anything, whatever they hold,
  * their outputs and gradients are zero, and the state is the one behind the row's last frame.  No operator keeps anything between
  * calls, uses atomics or clears memory with a memset: results are the same bits on every run and every call can be captured.  `ws` is
